@@ -82,6 +82,7 @@ void adam_step(at::Tensor p, at::Tensor g, at::Tensor m, at::Tensor v, at::Tenso
 
 void register_conv_ops(pybind11::module_& m);   // conv_bindings.cpp
 void register_stem_ops(pybind11::module_& m);   // stem_bindings.cpp
+void register_ffn_ops(pybind11::module_& m);    // ffn_bindings.cpp
 void register_reducer(pybind11::module_& m);    // reducer.cpp
 void register_p2p(pybind11::module_& m);        // p2p.cpp
 void register_io(pybind11::module_& m);         // png_loader.cpp
@@ -109,6 +110,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_rccl(m);          // first: RcclComm is a default-argument type of the reducer / P2P engine bindings
   register_conv_ops(m);
   register_stem_ops(m);
+  register_ffn_ops(m);
   register_reducer(m);
   register_p2p(m);
   register_io(m);

@@ -1,0 +1,110 @@
+// Products with few rows (inference on one or a few rows): out[m][n] = epilogue(sum_k w(n, k) x(m, k)), m < 32.
+//
+// Bound by reading the weights once: 2 N K bytes in 16 bits against 2 M N K operations.  A workgroup owns 16 weight rows and
+// streams them from memory straight into the matrix cores' A operand (lane: 16 bytes of one row), eight waves splitting k;
+// the few rows of x come out of L2 as the B operand.  The waves' sums meet in LDS in a fixed order, so the result does not
+// depend on timing.  With 16 rows a workgroup even N = 4096 gives every CU a workgroup of eight waves.
+// Rows of x beyond M repeat row 0 (their sums are dropped).
+#include "ffn_common.h"
+#include "ffn_mma.h"
+#include "ddl_kernels.h"
+
+namespace ddl {
+namespace ffn {
+namespace {
+
+constexpr int NW = 8, U = 4;
+
+template <typename T, bool VEC>
+__device__ __forceinline__ typename Mma<T>::Frag load_chunk(const T* row, int k, int K) {
+  using Frag = typename Mma<T>::Frag;
+  constexpr int EPC = 16 / sizeof(T);
+  Frag f;
+  if (VEC) {                                               // K is a multiple of the chunk: all of it or nothing
+    if (k < K) f = *reinterpret_cast<const Frag*>(row + k);
+    else f = Frag{};
+  } else {
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) f[e] = k + e < K ? row[k + e] : (T)0.f;
+  }
+  return f;
+}
+
+template <typename T, int MT, bool DUAL, bool VEC>
+__global__ void __launch_bounds__(NW * 64) few_rows_kernel(FewRowsArgs a) {
+  using Frag = typename Mma<T>::Frag;
+  constexpr int EPC = 16 / sizeof(T), KS = 4 * EPC;        // k of one step of a wave
+  constexpr int D = DUAL ? 2 : 1;
+  __shared__ float red[NW][D][MT * 16][16];
+  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, i = l & 15, kg = l >> 4;
+  const int n0 = blockIdx.x * 16, n = min(n0 + i, a.N - 1);
+  const T* w[D];
+  const T* x[MT];
+#pragma unroll
+  for (int d = 0; d < D; ++d) w[d] = (const T*)a.w[d] + (long)n * a.ldw[d];
+#pragma unroll
+  for (int u = 0; u < MT; ++u) x[u] = (const T*)a.x + (u * 16 + i < a.M ? (long)(u * 16 + i) * a.ldx : 0);
+
+  f32x4 acc[D][MT];
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+#pragma unroll
+    for (int u = 0; u < MT; ++u) acc[d][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int kb = wave * KS * U; kb < a.K; kb += NW * KS * U) {
+    Frag wf[D][U], xf[MT][U];
+#pragma unroll
+    for (int s = 0; s < U; ++s) {
+#pragma unroll
+      for (int d = 0; d < D; ++d) wf[d][s] = load_chunk<T, VEC>(w[d], kb + s * KS + kg * EPC, a.K);
+#pragma unroll
+      for (int u = 0; u < MT; ++u) xf[u][s] = load_chunk<T, VEC>(x[u], kb + s * KS + kg * EPC, a.K);
+    }
+#pragma unroll
+    for (int s = 0; s < U; ++s)
+#pragma unroll
+      for (int d = 0; d < D; ++d)
+#pragma unroll
+        for (int u = 0; u < MT; ++u) acc[d][u] = Mma<T>::mma(wf[d][s], xf[u][s], acc[d][u]);
+  }
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+#pragma unroll
+    for (int u = 0; u < MT; ++u) *reinterpret_cast<f32x4*>(&red[wave][d][u * 16 + i][4 * kg]) = acc[d][u];
+  __syncthreads();
+  const int o = threadIdx.x, m = o >> 4, nn = n0 + (o & 15);
+  if (o >= MT * 256 || m >= a.M || nn >= a.N) return;
+  float v = 0.f, v1 = 0.f;
+#pragma unroll
+  for (int q = 0; q < NW; ++q) {
+    v += red[q][0][m][o & 15];
+    if (DUAL) v1 += red[q][D - 1][m][o & 15];
+  }
+  float b0, b1;
+  load_bias<T, 1>(a.ep, 0, nn, a.N, &b0);
+  load_bias<T, 1>(a.ep, 1, nn, a.N, &b1);
+  epilogue_store<T, DUAL, false, 1>(a.ep, 0, m, nn, a.N, &v, &v1, &b0, &b1);
+}
+
+template <typename T, int MT, bool DUAL> void run_vec(const FewRowsArgs& a, hipStream_t s) {
+  const dim3 grid((a.N + 15) / 16), block(NW * 64);
+  if (a.vec) hipLaunchKernelGGL((few_rows_kernel<T, MT, DUAL, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((few_rows_kernel<T, MT, DUAL, false>), grid, block, 0, s, a);
+}
+template <typename T> void run(const FewRowsArgs& a, hipStream_t s) {
+  if (a.dual) {
+    if (a.M <= 16) run_vec<T, 1, true>(a, s); else run_vec<T, 2, true>(a, s);
+  } else {
+    if (a.M <= 16) run_vec<T, 1, false>(a, s); else run_vec<T, 2, false>(a, s);
+  }
+}
+}  // namespace
+
+void launch_few_rows(int dtype, const FewRowsArgs& a, hipStream_t s) {
+  if (dtype == F32) run<float>(a, s);
+  else if (dtype == BF16) run<__bf16>(a, s);
+  else run<_Float16>(a, s);
+  DDL_HIP_CHECK(hipGetLastError());
+}
+
+}  // namespace ffn
+}  // namespace ddl

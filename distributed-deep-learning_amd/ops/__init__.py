@@ -133,3 +133,9 @@ def adam_step_flat(p, g, m, v, step_t, aux_t, lr, b1, b2, eps, wd, zero_grad: bo
     ext = require_ext()
     ext.adam_step(p, g, m, v, step_t, aux_t, float(lr), float(b1), float(b2), float(eps), float(wd),
                   bool(zero_grad), [int(s) for s, _ in ranges], [int(e) for _, e in ranges])
+
+
+# --------------------------------------------------------------------------------------
+# feed-forward block: products with epilogues, gated block, dropout, residual + norms
+# --------------------------------------------------------------------------------------
+from .ffn import ACTIVATIONS, DropoutRng, dropout, gated_linear, linear, residual_norm  # noqa: E402,F401

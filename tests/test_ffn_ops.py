@@ -1,0 +1,99 @@
+"""Feed-forward operators on the CPU (plain PyTorch path): formulas, generator, refusals."""
+import pytest
+import torch
+
+import ffn_oracle as oracle
+from ddl import ops
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def rnd(dtype, *shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def same(got, want, dtype, size=1.0):
+    """64-bit value against one rounding plus fp32 arithmetic over at most 64 terms of `size`"""
+    assert got.dtype == dtype
+    off = (got.double() - want).abs()
+    assert (off <= oracle.rounding(dtype) * want.abs() + 128 * 2.0 ** -24 * (size + want.abs())).all(), off.max()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ops.ACTIVATIONS)
+def test_products(dtype, act):
+    x, w, u = rnd(dtype, 2, 5, 24, seed=1), rnd(dtype, 7, 24, seed=2), rnd(dtype, 7, 24, seed=3)
+    b, c, r = rnd(dtype, 7, seed=4), rnd(dtype, 7, seed=5), rnd(dtype, 2, 5, 7, seed=6)
+    d = [t.double() for t in (x, w, u, b, c, r)]
+    size = (d[0].abs() @ d[1].abs().T).max().item() * (d[0].abs() @ d[2].abs().T).max().item()
+    same(ops.linear(x, w, b, activation=act, residual=r), oracle.linear(d[0], d[1], d[3], act, d[5]), dtype, size)
+    same(ops.gated_linear(x, w, u, b, c, activation=act), oracle.gated(d[0], d[1], d[2], d[3], d[4], act), dtype, size)
+    for t in (x, w, b, r):
+        t.requires_grad_(True)
+    ops.linear(x, w, b, activation=act, residual=r).sum().backward()
+    assert all(t.grad is not None and t.grad.dtype == dtype for t in (x, w, b, r))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("post", [True, False])
+@pytest.mark.parametrize("gate", ["none", "channel", "full"])
+def test_residual_norm(dtype, kind, post, gate):
+    x, y = rnd(dtype, 3, 4, 40, seed=1), rnd(dtype, 3, 4, 40, seed=2)
+    a = dict(pre_weight=rnd(dtype, 40, seed=3), post_weight=rnd(dtype, 40, seed=4) if post else None,
+             gate={"none": None, "channel": rnd(dtype, 40, seed=5), "full": rnd(dtype, 3, 4, 40, seed=5)}[gate])
+    if kind == "layer":
+        a["pre_bias"] = rnd(dtype, 40, seed=6)
+    r, h = ops.residual_norm(x, y, kind=kind, scale=0.5, **a)
+    wr, wh = oracle.residual_norm(x.double(), y.double(), kind=kind, scale=0.5, **{k: v.double() if v is not None else None for k, v in a.items()})
+    same(r, wr, dtype, 30.0)
+    same(h, wh, dtype, 30.0)
+    r, h = ops.residual_norm(x, kind=kind, pre_weight=a["pre_weight"])
+    assert r is x
+    same(h, oracle.norm(x.double(), a["pre_weight"].double(), None, kind, 1e-6), dtype, 30.0)
+
+
+def test_generator_known_answers():
+    """Philox4x32 with 10 and 7 rounds on the zero block, as published with the generator."""
+    assert oracle.philox4x32((0,) * 4, (0, 0), 10) == (0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8)
+    assert oracle.philox4x32((0,) * 4, (0, 0), 7) == (0x5f6fb709, 0x0d893f64, 0x4f121f81, 0x4f730a48)
+
+
+@pytest.mark.parametrize("n", [0, 1, 5, 64, 1001])
+@pytest.mark.parametrize("p", [0.0, 0.25, 1.0])
+def test_dropout(n, p):
+    for key in [(0, 0), (-5, 2 ** 50 + 3), (2 ** 62, 9)]:
+        keep = torch.from_numpy(oracle.kept(key, n, p)).double()
+        x, res = rnd(torch.float32, n, seed=1).requires_grad_(True), rnd(torch.float32, n, seed=2)
+        y = ops.dropout(x, p, torch.tensor(key), residual=res)
+        scale = 1 / (1 - p) if p < 1 else 0.0
+        same(y.detach(), x.detach().double() * keep * scale + res.double(), torch.float32, 4.0)
+        (dx,) = torch.autograd.grad(y.sum(), x)
+        same(dx, keep * scale, torch.float32)
+    bad = torch.full((1000,), float("nan"))
+    assert (ops.dropout(bad, 1.0, torch.tensor([1, 2])) == 0).all()
+
+
+def test_dropout_rng():
+    rng = ops.DropoutRng(2 ** 63 + 5, "cpu", stream=2)
+    assert rng.keys(2).tolist() == [[5 - 2 ** 63, 2 << 48], [5 - 2 ** 63, (2 << 48) + 1]]
+    assert rng.next_key().tolist() == [5 - 2 ** 63, (2 << 48) + 2]
+
+
+def test_refusals():
+    x, w, b, n, key = rnd(torch.float32, 4, 8), rnd(torch.float32, 6, 8), rnd(torch.float32, 6), torch.ones(8), torch.tensor([1, 2])
+    bad = [
+        lambda: ops.linear(x, w[:, :7]), lambda: ops.linear(x, w.bfloat16()), lambda: ops.linear(x, w, b[:5]),
+        lambda: ops.linear(x, w, b, residual=x), lambda: ops.linear(x.double(), w.double()), lambda: ops.linear(x, w, activation="tanh"),
+        lambda: ops.gated_linear(x, w, w[:5]), lambda: ops.gated_linear(x, w, w, b), lambda: ops.dropout(x, 1.5, key),
+        lambda: ops.dropout(x, 0.5, key[:1]), lambda: ops.dropout(x, 0.5, key.float()), lambda: ops.dropout(x, 0.5, key, residual=w),
+        lambda: ops.DropoutRng(0, "cpu", stream=-1), lambda: ops.residual_norm(x), lambda: ops.residual_norm(x, gate=n, pre_weight=n),
+        lambda: ops.residual_norm(x, x[:3]), lambda: ops.residual_norm(x, pre_weight=n, pre_bias=n),
+        lambda: ops.residual_norm(x, x, kind="batch"), lambda: ops.residual_norm(x, x, pre_weight=n[:7]),
+        lambda: ops.residual_norm(x, x, pre_weight=n, gate=n.half()), lambda: ops.residual_norm(x, x, gate=x[:2]),
+        lambda: ops.residual_norm(x, x, eps=-1.0),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")

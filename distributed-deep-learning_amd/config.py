@@ -53,6 +53,9 @@ class TrainConfig:
     max_steps: int = 0                  # >0: stop each epoch after this many steps (smoke runs)
     # ---- model ---------------------------------------------------------------
     dtype: str = "fp32"                 # fp32 (reference parity) | bf16 (mixed: bf16 MFMA inputs)
+    head: str = "linear"                # linear (the reference's) | gated: a residual feed-forward block in front of it
+    head_width: int = 1024              # gated: hidden columns
+    head_dropout: float = 0.1           # gated: dropout on the block's output in training
     hip_graph: bool = True              # capture the native train step into a hipGraph
     pretrained: Optional[str] = field(default_factory=lambda: os.environ.get("DDL_PRETRAINED") or None)
     #   ^ torchvision densenet121 state-dict file (reference: weights=IMAGENET1K_V1, single.py:297)
@@ -107,6 +110,11 @@ class TrainConfig:
 
     def replace(self, **kw: Any) -> "TrainConfig":
         return dataclasses.replace(self, **kw)
+
+    def head_config(self):
+        from .models.head import HeadConfig
+
+        return HeadConfig(self.head, self.head_width, self.head_dropout)
 
     @property
     def ckpt_subdir(self) -> str:

@@ -706,4 +706,14 @@ void register_ffn_ops(pybind11::module_& m) {
   m.def("dropout", &dropout);
   m.def("rng_keys", &rng_keys, "state (seed, calls) -> n keys (seed, call); calls += n");
   m.def("residual_norm", &residual_norm);
+  m.def("norm_forward", [](const Tensor& x, const OptT& y, const OptT& gate, const OptT& post_w, const OptT& post_b, const OptT& pre_w,
+                           const OptT& pre_b, bool layer, double eps, double scale) {
+    return norm_forward(norm_in(x, y, gate, post_w, post_b, pre_w, pre_b, layer, eps, scale), true);
+  }, "-> (r, h, statistics)");
+  m.def("norm_backward", [](const Tensor& x, const OptT& y, const OptT& gate, const OptT& post_w, const OptT& post_b, const OptT& pre_w,
+                            const OptT& pre_b, bool layer, double eps, double scale, const Tensor& stats, const OptT& dr, const OptT& dh) {
+    const NormIn in = norm_in(x, y, gate, post_w, post_b, pre_w, pre_b, layer, eps, scale);
+    NormGrads g = norm_backward(in, stats, get(dr), get(dh), true, has(y), has(gate), has(post_w), has(post_b), has(pre_w), has(pre_b));
+    return std::make_tuple(g.dx, g.dy, g.v[0], g.v[1], g.v[2], g.v[3], g.v[4]);
+  }, "-> (dx, dbranch, dgate, dpost_w, dpost_b, dpre_w, dpre_b)");
 }

@@ -7,10 +7,11 @@ import torch
 
 from .densenet import (UNIT_NAMES, DenseNetStage, build_stage, default_split_points, densenet121,
                        stage_units)
+from .head import HeadConfig
 
 
 def create_stage(units: Sequence[str], device, num_classes: int = 5, dtype: str = "fp32",
-                 pretrained: str = None, **native_kw) -> torch.nn.Module:
+                 pretrained: str = None, head: HeadConfig = HeadConfig(), **native_kw) -> torch.nn.Module:
     """A contiguous run of DenseNet-121 units on ``device``.
 
     The device decides the implementation - there is no user-selectable backend: on a GPU a stage IS the
@@ -19,11 +20,11 @@ def create_stage(units: Sequence[str], device, num_classes: int = 5, dtype: str 
     numerics oracle the GPU tests instantiate directly (``DenseNetStage(...).to(device)``)."""
     device = torch.device(device)
     if device.type != "cuda":
-        stage = DenseNetStage(units, num_classes).to(device)
+        stage = DenseNetStage(units, num_classes, head).to(device)
     else:
         from .native_densenet import NativeDenseNetStage
 
-        stage = NativeDenseNetStage(units, num_classes=num_classes, device=device, dtype=dtype, **native_kw)
+        stage = NativeDenseNetStage(units, num_classes=num_classes, device=device, dtype=dtype, head=head, **native_kw)
     if pretrained:
         # reference: densenet121(weights=IMAGENET1K_V1) + a fresh Linear(1024, classes) (single.py:297-299)
         from .pretrained import load_pretrained

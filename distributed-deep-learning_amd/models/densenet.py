@@ -30,6 +30,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .head import GatedHead, HeadConfig
+
 GROWTH = 32
 BN_SIZE = 4
 BLOCK_CONFIG = (6, 12, 24, 16)
@@ -170,7 +172,7 @@ class DenseNetStage(nn.Module):
     single-model key space.
     """
 
-    def __init__(self, units: Sequence[str] = UNIT_NAMES, num_classes: int = 5) -> None:
+    def __init__(self, units: Sequence[str] = UNIT_NAMES, num_classes: int = 5, head: HeadConfig = HeadConfig()) -> None:
         super().__init__()
         units = tuple(units)
         atoms, mine = model_atoms(), unit_atoms(units)
@@ -199,6 +201,8 @@ class DenseNetStage(nn.Module):
                 feats["norm5"] = nn.BatchNorm2d(chans[-1][1])
         self.features = nn.Sequential(feats)
         if "head" in units:
+            if head.kind == "gated":
+                self.ffn = GatedHead(chans[-1][1], head)
             self.classifier = nn.Linear(chans[-1][1], num_classes)
         _init_weights(self)
 
@@ -218,6 +222,8 @@ class DenseNetStage(nn.Module):
             x = F.relu(x, inplace=True)
             x = F.adaptive_avg_pool2d(x, (1, 1))
             x = torch.flatten(x, 1)
+            if hasattr(self, "ffn"):
+                x = self.ffn(x)
             x = self.classifier(x)
         return x
 

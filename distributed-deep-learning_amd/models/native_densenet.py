@@ -44,6 +44,7 @@ from .. import ops
 from ..utils.arena import FlatArena, FlatBuffers, reverse_named_parameters
 from ..utils.knobs import knob
 from ..utils.streams import new_stream
+from . import head as gated_head
 from .densenet import (BLOCK_CONFIG, BN_SIZE, GROWTH, UNIT_NAMES, DenseNetStage, block_channels, parse_unit)
 
 BN_MOMENTUM = 0.1
@@ -505,22 +506,30 @@ class _HeadFn(torch.autograd.Function):
         ext.bn_prep(None, 0, 0, float(M), stats[0], stats[1], stats[2], unit.g, unit.b, unit.rm, unit.rv,
                     ss[0], ss[1], C, BN_MOMENTUM, BN_EPS, train, **pend)
         pooled = ext.bnrelu_gap_fwd(buf2d, B, H * W, ss[0], ss[1])
+        ffn = ()
+        if unit.ffn is not None:             # residual feed-forward block in front of the classifier (models/head.py)
+            key = unit.stage.dropout_key() if train and unit.drop > 0 else None
+            pooled, ffn = gated_head.native_forward(ext, unit.ffn, pooled, unit.drop, key)
+            ffn += () if key is None else (key,)
         logits = ext.linear_fwd(pooled, unit.cw, unit.cb)
         ctx.unit = unit
         ctx.geom = (B, H, W, C)
-        ctx.save_for_backward(buf, stats, ss, pooled)
+        ctx.save_for_backward(buf, stats, ss, pooled, *ffn)
         return logits
 
     @staticmethod
     def backward(ctx, dlogits: torch.Tensor):
         ext = _ext()
         unit = ctx.unit
-        buf, stats, ss, pooled = ctx.saved_tensors
+        buf, stats, ss, pooled, *ffn = ctx.saved_tensors
         B, H, W, C = ctx.geom
         M = B * H * W
         f32 = dict(dtype=torch.float32, device=buf.device)
         buf2d = buf.view(M, C)
         dpooled = ext.linear_bwd(dlogits.contiguous(), pooled, unit.cw, unit.gcw, unit.gcb)
+        if unit.ffn is not None:
+            dpooled, grads = gated_head.native_backward(ext, unit.ffn, ffn[:7], unit.drop, ffn[7] if len(ffn) > 7 else None, dpooled)
+            torch._foreach_add_(unit.gffn, grads)
         dbuf = torch.empty(B, H, W, C, **f32)
         d2d = dbuf.view(M, C)
         st = ext.rows_op(3, M, dpooled, buf2d, ss[0], ss[1], d2d, H, W, True)
@@ -549,6 +558,13 @@ class HeadUnit:
         self.cb, self.gcb = st.pv("classifier.bias")
         self.rm, self.rv = st.bv("features.norm5.running_mean"), st.bv("features.norm5.running_var")
         self.param_names = ["features.norm5.weight", "features.norm5.bias", "classifier.weight", "classifier.bias"]
+        self.ffn, self.gffn, self.drop = None, None, 0.0
+        if st.head.kind == "gated":
+            views = {n: st.pv("ffn." + n) for n in gated_head.PARAMS}
+            self.ffn = {n: v[0] for n, v in views.items()}
+            self.gffn = [v[1] for v in views.values()]
+            self.drop = st.head.dropout
+            self.param_names += ["ffn." + n for n in gated_head.PARAMS]
 
     def __call__(self, x, in_stats):
         return _HeadFn.apply(x, self.stage.anchor, self, in_stats), None
@@ -607,7 +623,8 @@ class NativeDenseNetStage(nn.Module):
 
     def __init__(self, units: Sequence[str] = UNIT_NAMES, num_classes: int = 5, device="cuda",
                  dtype: str = "fp32", bucket_mb: float = 8.0, dp_world: int = 1,
-                 wgrad_min_rows: int = 64, grad_phases: Sequence[str] = ()) -> None:
+                 wgrad_min_rows: int = 64, grad_phases: Sequence[str] = (),
+                 head: gated_head.HeadConfig = gated_head.HeadConfig()) -> None:
         super().__init__()
         if dtype not in ("fp32", "bf16", "fp32x3"):
             raise ValueError(f"dtype must be fp32, bf16 or fp32x3, got {dtype!r}")
@@ -644,9 +661,12 @@ class NativeDenseNetStage(nn.Module):
         self.units = tuple(units)
         self.num_classes = num_classes
         self.wgrad_min_rows = wgrad_min_rows
-        ref = DenseNetStage(self.units, num_classes)          # same init distribution as the reference
+        self.head = head
+        ref = DenseNetStage(self.units, num_classes, head)    # same init distribution as the reference
         self.features = ref.features
         if "head" in self.units:
+            if head.kind == "gated":
+                self.ffn = ref.ffn
             self.classifier = ref.classifier
         # re-lay-out conv weights for the MFMA kernels
         for name, mod in self.named_modules():
@@ -706,6 +726,11 @@ class NativeDenseNetStage(nn.Module):
         # zeros) and the running statistics are advanced in micro-batch order afterwards (``combine_buffer_lanes``)
         self._buf_lanes: List[torch.Tensor] = [self.flat_buffers.flat_float]
         self._buf_lane = 0
+        # dropout keys of the gated head: one generator per buffer lane, so that concurrent micro-batch forwards draw the keys
+        # they would draw one after the other
+        self._dropout_seed = gated_head.dropout_seed()
+        self._dropout_rngs: List[ops.DropoutRng] = []
+        self._ensure_dropout_rngs()
         self.defer_counters = False       # num_batches_tracked advanced by combine_buffer_lanes instead of per forward
         self._mb_forwarded = set()
         for u in self.unit_objs:
@@ -716,7 +741,7 @@ class NativeDenseNetStage(nn.Module):
 
     def unit_of_param(self, fqn: str) -> str:
         """Unit of this stage that owns a parameter (torchvision FQN)."""
-        if fqn.startswith("classifier.") or fqn.startswith("features.norm5."):
+        if fqn.startswith(("classifier.", "features.norm5.", "ffn.")):
             return "head"
         parts = fqn.split(".")
         part = parts[1]
@@ -807,7 +832,15 @@ class NativeDenseNetStage(nn.Module):
     def ensure_buffer_lanes(self, n_microbatches: int) -> None:
         while len(self._buf_lanes) < 1 + n_microbatches:
             self._buf_lanes.append(torch.zeros_like(self.flat_buffers.flat_float))
+        self._ensure_dropout_rngs()
         self.defer_counters = True
+
+    def _ensure_dropout_rngs(self) -> None:
+        while "head" in self.units and self.head.kind == "gated" and len(self._dropout_rngs) < len(self._buf_lanes):
+            self._dropout_rngs.append(ops.DropoutRng(self._dropout_seed, self.anchor.device, stream=len(self._dropout_rngs)))
+
+    def dropout_key(self) -> torch.Tensor:
+        return self._dropout_rngs[self._buf_lane].next_key()
 
     def begin_microbatch_buffers(self, i: int) -> None:
         """Training forward of micro-batch ``i`` is next (eager, or being captured): its BN kernels update scratch

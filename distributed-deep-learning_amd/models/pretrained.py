@@ -68,8 +68,8 @@ def load_pretrained(stage: torch.nn.Module, path: str, verbose: bool = True) -> 
     if not loaded:
         raise ValueError(f"{path}: no tensor matched this model (not a DenseNet-121 state-dict?)")
     if verbose:
-        head = [k for k in skipped if k.startswith("classifier.")]
-        other = [k for k in skipped if not k.startswith("classifier.")]
+        head = [k for k in skipped if k.startswith(("classifier.", "ffn."))]
+        other = [k for k in skipped if k not in head]
         print(f"pretrained: {len(loaded)} tensors from {path}"
               + (f"; fresh classifier ({len(head)} tensors)" if head else "")
               + (f"; NOT found: {other[:4]}{'...' if len(other) > 4 else ''}" if other else ""), flush=True)

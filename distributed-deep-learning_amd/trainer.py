@@ -118,7 +118,7 @@ class SingleStrategy(Strategy):
     def __init__(self, cfg, ctx) -> None:
         super().__init__(cfg, ctx)
         self.model = create_stage(UNIT_NAMES, self.device, cfg.num_classes, cfg.dtype,
-                                  pretrained=cfg.pretrained)
+                                  pretrained=cfg.pretrained, head=cfg.head_config())
         self.arena = _arena_for(self.model, self.device, cfg.bucket_mb, 1)
         self.optimizer = self._make_optimizer(self.arena)
         self.global_rank = self.local_rank = 0          # single.py:269 hard-codes 0,0
@@ -144,7 +144,7 @@ class DDPStrategy(Strategy):
     def __init__(self, cfg, ctx, group=None) -> None:
         super().__init__(cfg, ctx)
         self.model = create_stage(UNIT_NAMES, self.device, cfg.num_classes, cfg.dtype,
-                                  pretrained=cfg.pretrained, **self._native_kw(cfg, comm.get_world_size(group)))
+                                  pretrained=cfg.pretrained, head=cfg.head_config(), **self._native_kw(cfg, comm.get_world_size(group)))
         self.dp = DataParallelEngine(self.model, group=group, device=self.device, bucket_mb=cfg.bucket_mb,
                                      grad_sync=cfg.grad_sync, sync_buffers=cfg.sync_buffers,
                                      zero1=cfg.zero1, profiler=self.profiler, debug_sync=cfg.debug_sync, rccl=cfg.rccl)
@@ -228,7 +228,7 @@ class PPStrategy(Strategy):
             phases = tuple(u for u in self.units if u.startswith("denseblock")) if (hybrid and cfg.hip_graph) else ()
             nat = dict(bucket_mb=cfg.bucket_mb, dp_world=mesh.dp_size, grad_phases=phases)
         self.model = create_stage(self.units, self.device, cfg.num_classes, cfg.dtype,
-                                  pretrained=cfg.pretrained, **nat)
+                                  pretrained=cfg.pretrained, head=cfg.head_config(), **nat)
         self.name = "ddpnpp" if hybrid else "pp"
         if hybrid:
             self.dp = DataParallelEngine(self.model, group=mesh.get_group("dp"), device=self.device,

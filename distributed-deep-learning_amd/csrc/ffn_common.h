@@ -122,20 +122,20 @@ template <int V> __device__ __forceinline__ void act_fwd_all(int act, float* v) 
 }
 
 // bias of the columns n .. n+V-1 (zeros where there is none)
-template <typename T, int V> __device__ __forceinline__ void load_bias(const Epilogue& e, int which, int n, int N, float* b) {
+template <typename T, int V> __device__ __forceinline__ void load_bias(const Epilogue& e, int which, int n, int N, bool aligned, float* b) {
 #pragma unroll
   for (int i = 0; i < V; ++i) b[i] = 0.f;
-  if (e.bias[which] != nullptr && n < N) load_some<T, V>((const T*)e.bias[which] + n, b, N - n, N - n >= V && e.bias_vec);
+  if (e.bias[which] != nullptr && n < N) load_some<T, V>((const T*)e.bias[which] + n, b, N - n, N - n >= V && aligned && e.bias_vec);
 }
 
 // V consecutive outputs (row m, columns n .. n+V-1); v: the sums, w: the second product's (dual only); b0, b1: their biases.
-// z rows are padded to 16 values, so z is stored in whole vectors.  PLAIN: neither bias, activation nor residual.
+// z rows are padded to 16 values, so z is stored in whole vectors where n is `aligned` (to the vector).  PLAIN: neither bias, activation nor residual.
 template <typename T, bool DUAL, bool PLAIN, int V>
-__device__ __forceinline__ void epilogue_store(const Epilogue& e, int which, long m, int n, int N, float* v, float* w,
+__device__ __forceinline__ void epilogue_store(const Epilogue& e, int which, long m, int n, int N, bool aligned, float* v, float* w,
                                                const float* b0, const float* b1) {
   const int left = N - n;
   if (left <= 0) return;
-  const bool full = left >= V;
+  const bool full = left >= V && aligned;
   if (!PLAIN) {
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] += b0[i];
@@ -144,8 +144,8 @@ __device__ __forceinline__ void epilogue_store(const Epilogue& e, int which, lon
       for (int i = 0; i < V; ++i) w[i] += b1[i];
     }
     if (e.z[0] != nullptr) {
-      store_vec<float, V>(e.z[0] + m * e.ldz + n, v);
-      if (DUAL) store_vec<float, V>(e.z[1] + m * e.ldz + n, w);
+      store_some<float, V>(e.z[0] + m * e.ldz + n, v, left, aligned);
+      if (DUAL) store_some<float, V>(e.z[1] + m * e.ldz + n, w, left, aligned);
     }
     act_fwd_all<V>(e.act, v);
     if (DUAL) {

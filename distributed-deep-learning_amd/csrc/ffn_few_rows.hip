@@ -80,9 +80,9 @@ __global__ void __launch_bounds__(NW * 64) few_rows_kernel(FewRowsArgs a) {
     if (DUAL) v1 += red[q][D - 1][m][o & 15];
   }
   float b0, b1;
-  load_bias<T, 1>(a.ep, 0, nn, a.N, &b0);
-  load_bias<T, 1>(a.ep, 1, nn, a.N, &b1);
-  epilogue_store<T, DUAL, false, 1>(a.ep, 0, m, nn, a.N, &v, &v1, &b0, &b1);
+  load_bias<T, 1>(a.ep, 0, nn, a.N, true, &b0);
+  load_bias<T, 1>(a.ep, 1, nn, a.N, true, &b1);
+  epilogue_store<T, DUAL, false, 1>(a.ep, 0, m, nn, a.N, true, &v, &v1, &b0, &b1);
 }
 
 template <typename T, int MT, bool DUAL> void run_vec(const FewRowsArgs& a, hipStream_t s) {

@@ -4,9 +4,9 @@
 namespace ddl {
 namespace ffn {
 void launch_gemm_bf16(const GemmArgs& a, int cfg, hipStream_t s) {
-  if (cfg == 0) run_cfg<__bf16, 64, 32, 1, 1>(a, s);
+  if (cfg == 0) run_cfg<__bf16, 128, 32, 2, 1>(a, s);
   else if (cfg == 1) run_cfg<__bf16, 128, 128, 2, 2>(a, s);
-  else run_cfg<__bf16, 256, 256, 4, 2>(a, s);
+  else run_big<__bf16>(a, s);
 }
 }  // namespace ffn
 }  // namespace ddl

@@ -5,7 +5,7 @@
 namespace ddl {
 namespace ffn {
 void launch_gemm_f32(const GemmArgs& a, int cfg, hipStream_t s) {
-  if (cfg == 0) run_cfg<float, 64, 32, 1, 1>(a, s);
+  if (cfg == 0) run_cfg<float, 128, 32, 2, 1>(a, s);
   else run_cfg<float, 128, 128, 2, 2>(a, s);
 }
 }  // namespace ffn

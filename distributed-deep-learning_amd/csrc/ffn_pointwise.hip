@@ -48,9 +48,9 @@ __global__ void __launch_bounds__(256) join_kernel(GemmArgs a) {
       }
       p += planes * plane;
     }
-    load_bias<T, V>(a.ep, 0, n, a.N, b0);
-    load_bias<T, V>(a.ep, 1, n, a.N, b1);
-    epilogue_store<T, DUAL, false, V>(a.ep, which, m, n, a.N, v, w, b0, b1);
+    load_bias<T, V>(a.ep, 0, n, a.N, true, b0);
+    load_bias<T, V>(a.ep, 1, n, a.N, true, b1);
+    epilogue_store<T, DUAL, false, V>(a.ep, which, m, n, a.N, true, v, w, b0, b1);
   }
 }
 
@@ -202,10 +202,12 @@ GemmPlan gemm_plan(int dtype, const GemmArgs& a) {
   };
   GemmPlan p;
   p.ldw = (a.N + 15) / 16 * 16;
-  if (dtype != F32 && tiles(256, 256) >= 192) p.cfg = 2;
+  const bool same = a.nseg == 1 || (a.ldp[0] == a.ldp[1] && a.ldq[0] == a.ldq[1]);
+  const bool holds = a.M >= 256 && a.N >= (a.dual ? 128 : 256) && same;
+  if (dtype != F32 && holds && tiles(256, 256) >= 192) p.cfg = 2;
   else if (a.M > 64) p.cfg = 1;
   else p.cfg = 0;
-  const long t = p.cfg == 2 ? tiles(256, 256) : p.cfg == 1 ? tiles(128, 128) : tiles(64, 32);
+  const long t = p.cfg == 2 ? tiles(256, 256) : p.cfg == 1 ? tiles(128, 128) : tiles(128, 32);
   const int tk = 128 / esize(dtype);
   const long slabs = (long)((a.K + tk - 1) / tk) * a.nseg;
   const long want = p.cfg == 2 ? 1 : (p.cfg == 1 ? 384 : 1024) / (t < 1 ? 1 : t);

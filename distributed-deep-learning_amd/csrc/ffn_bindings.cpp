@@ -58,25 +58,33 @@ bool rows_aligned(const Tensor& t) {
 }
 
 // An operand of a product: 16-byte aligned rows of whole 16-byte chunks.  A tensor that is not laid out so (odd widths, a column
-// slice, a transposed view) is packed into a padded copy, one pass over it.
+// slice, a transposed view) is packed into a copy whose rows are padded with zeros to 128 bytes, one pass over it.  Training
+// keeps the copy instead of the tensor, so the backward pass finds it packed: [rows, padded] with the width known from elsewhere.
 struct Operand {
   Tensor keep;
   const void* p = nullptr;
   long ld = 0;
 };
+long line(int64_t n, const Tensor& like) { return up(n, 128 / like.element_size()); }
 bool is_operand(const Tensor& t) {
   const int64_t epc = 16 / t.element_size();
   return t.numel() == 0 || ((t.size(1) <= 1 || t.stride(1) == 1) && t.size(1) % epc == 0 && rows_aligned(t));
 }
-Operand operand(const Tensor& t, int dtype) {                       // t: 2-D
+Operand operand(const Tensor& t, int dtype, int64_t width) {        // t: 2-D [rows, width], or packed already
   Operand o;
+  if (t.size(1) != width) {
+    o.keep = t;
+    o.p = t.data_ptr();
+    o.ld = t.size(1);
+    return o;
+  }
   if (is_operand(t)) {
     o.keep = t;
     o.p = t.numel() ? t.data_ptr() : nullptr;
     o.ld = row_stride(t);
     return o;
   }
-  o.ld = up(t.size(1), 16);
+  o.ld = line(t.size(1), t);
   o.keep = at::empty({t.size(0), o.ld}, t.options());
   ffn::launch_pack(dtype, t.data_ptr(), t.stride(0), t.stride(1), o.keep.data_ptr(), o.ld, t.size(0), (int)t.size(1), cur_stream());
   o.p = o.keep.data_ptr();
@@ -127,16 +135,21 @@ std::vector<int64_t> out_sizes(const Tensor& x, int64_t n) {
   return s;
 }
 
-// One or two weights.  Returns out [M, N] and the fp32 sums z (one or two planes [M, ldz]) if `keep`.
-std::pair<Tensor, Tensor> product_forward(const Tensor& x, const Tensor& w0, const Tensor& w1, const Tensor& b0, const Tensor& b1,
-                                          const Tensor& res, int act, bool keep, const char* op) {
+// What a product keeps for its backward pass: the fp32 sums z (one or two planes [M, ldz]; none without an activation), and x and the
+// weights as they were packed (otherwise as given).
+struct Kept { Tensor z, x, w[2]; };
+
+// One or two weights -> out [M, N].
+Tensor product_forward(const Tensor& x, const Tensor& w0, const Tensor& w1, const Tensor& b0, const Tensor& b1, const Tensor& res,
+                       int act, bool keep_sums, Kept* kept, const char* op) {
   const int dtype = type_of(x, op);
   const Tensor x2 = rows_of(x);
   const int M = dim_of(x2.size(0), op), K = dim_of(x2.size(1), op), N = dim_of(w0.size(0), op);
   const bool dual = w1.defined();
   Tensor out = at::empty({M, N}, x.options()), z;
-  if (keep) z = at::empty({dual ? 2 : 1, M, up(N, 16)}, x.options().dtype(at::kFloat));
-  if (M == 0 || N == 0) return {out, z};
+  if (keep_sums) z = at::empty({dual ? 2 : 1, M, up(N, 16)}, x.options().dtype(at::kFloat));
+  if (kept != nullptr) *kept = {z, x, {w0, w1}};
+  if (M == 0 || N == 0) return out;
   ffn::Epilogue e;
   set_out(e, 0, out);
   e.act = act;
@@ -150,7 +163,7 @@ std::pair<Tensor, Tensor> product_forward(const Tensor& x, const Tensor& w0, con
     e.ldr = row_stride(r2);
     e.res_vec = rows_aligned(r2);
   }
-  if (keep) {
+  if (keep_sums) {
     e.ldz = z.size(2);
     e.z[0] = z.data_ptr<float>();
     if (dual) e.z[1] = e.z[0] + (long)M * e.ldz;
@@ -173,9 +186,14 @@ std::pair<Tensor, Tensor> product_forward(const Tensor& x, const Tensor& w0, con
       f.ldx = row_stride(x2);
     }
     ffn::launch_few_rows(dtype, f, cur_stream());
-    return {out, z};
+    return out;
   }
-  const Operand xo = operand(x2, dtype), wo = operand(w0, dtype), vo = dual ? operand(w1, dtype) : Operand();
+  const Operand xo = operand(x2, dtype, K), wo = operand(w0, dtype, K), vo = dual ? operand(w1, dtype, K) : Operand();
+  if (kept != nullptr) {
+    if (xo.keep.size(1) != K) kept->x = xo.keep;
+    if (wo.keep.size(1) != K) kept->w[0] = wo.keep;
+    if (dual && vo.keep.size(1) != K) kept->w[1] = vo.keep;
+  }
   ffn::GemmArgs g;
   g.N = N; g.M = M; g.K = K;
   g.dual = dual;
@@ -184,16 +202,17 @@ std::pair<Tensor, Tensor> product_forward(const Tensor& x, const Tensor& w0, con
   g.q[0] = xo.p; g.ldq[0] = xo.ld;
   g.ep = e;
   run_gemm(dtype, g, x);
-  return {out, z};
+  return out;
 }
 
-// Gradients of a product with one or two weights from dy [M, N] and what the forward pass kept.
+// Gradients of a product with one or two weights [N, K] from dy [.., N] and what the forward pass kept.
 struct ProductGrads { Tensor dx, dw[2], db[2]; };
-ProductGrads product_backward(const Tensor& dy, const Tensor& x, const Tensor& w0, const Tensor& w1, const Tensor& z, int act,
-                              bool need_dx, bool need_dw, bool need_db, const char* op) {
+ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width, int act, bool need_dx, bool need_dw, bool need_db,
+                              const char* op) {
+  const Tensor &x = kept.x, &w0 = kept.w[0], &w1 = kept.w[1], &z = kept.z;
   const int dtype = type_of(x, op);
   const Tensor x2 = rows_of(x), dy2 = rows_of(dy);
-  const int M = dim_of(x2.size(0), op), K = dim_of(x2.size(1), op), N = dim_of(w0.size(0), op);
+  const int M = dim_of(dy2.size(0), op), K = dim_of(width, op), N = dim_of(dy2.size(1), op);
   const bool dual = w1.defined();
   const int D = dual ? 2 : 1;
   ProductGrads r;
@@ -215,10 +234,10 @@ ProductGrads product_backward(const Tensor& dy, const Tensor& x, const Tensor& w
   Tensor dz;
   Operand dzo[2];
   if (make_dz) {
-    dz = at::empty({D, M, up(N, 16)}, x.options());
+    dz = at::empty({D, M, line(N, x)}, x.options());
     for (int d = 0; d < D; ++d) dzo[d] = own_operand(dz[d]);
   } else if (need_dx || need_dw) {
-    dzo[0] = operand(dy2, dtype);
+    dzo[0] = operand(dy2, dtype, N);
   }
   if (make_dz || need_db) {
     ffn::ActBwdArgs b;
@@ -228,7 +247,8 @@ ProductGrads product_backward(const Tensor& dy, const Tensor& x, const Tensor& w
     b.act = act;
     b.dual = dual;
     b.M = M; b.N = N;
-    b.ldd = b.ldz = up(N, 16);
+    b.ldd = line(N, x);
+    b.ldz = up(N, 16);
     Tensor part;
     if (z.defined())
       for (int d = 0; d < D; ++d) {
@@ -236,19 +256,22 @@ ProductGrads product_backward(const Tensor& dy, const Tensor& x, const Tensor& w
         if (make_dz) b.dz[d] = const_cast<void*>(dzo[d].p);
       }
     b.chunks = ffn::act_bwd_chunks(dtype, M, N);
-    if (need_db) {
+    void* outs[2] = {need_db ? r.db[0].data_ptr() : nullptr, need_db && dual ? r.db[1].data_ptr() : nullptr};
+    if (need_db && b.chunks == 1) {
+      b.db[0] = outs[0];
+      b.db[1] = outs[1];
+    } else if (need_db) {
       part = at::empty({b.chunks, D, N}, x.options().dtype(at::kFloat));
       b.part = part.data_ptr<float>();
     }
     ffn::launch_act_bwd(dtype, b, cur_stream());
-    if (need_db) {
-      void* outs[2] = {r.db[0].data_ptr(), dual ? r.db[1].data_ptr() : nullptr};
+    if (b.part != nullptr) {
       ffn::launch_colsum(dtype, b.part, b.chunks, D, N, outs, cur_stream());
     }
   }
   if (K == 0) return r;
   if (need_dx) {                                                     // dx[m][k] = sum over weights, n of dz[m][n] w[n][k]
-    const Operand wo[2] = {operand(w0, dtype), dual ? operand(w1, dtype) : Operand()};
+    const Operand wo[2] = {operand(rows_of(w0), dtype, K), dual ? operand(rows_of(w1), dtype, K) : Operand()};
     ffn::GemmArgs g;
     g.N = K; g.M = M; g.K = N;
     g.nseg = D;
@@ -261,7 +284,7 @@ ProductGrads product_backward(const Tensor& dy, const Tensor& x, const Tensor& w
     run_gemm(dtype, g, x);
   }
   if (need_dw) {                                                     // dw[n][k] = sum over m of dz[m][n] x[m][k]
-    const Operand xo = operand(x2, dtype);
+    const Operand xo = operand(x2, dtype, K);
     ffn::GemmArgs g;
     g.N = K; g.M = N; g.K = M;
     g.nout = D;
@@ -299,8 +322,9 @@ void check_linear(const Tensor& x, const Tensor& w, const OptT& b, const OptT& r
 std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, const OptT& b, const OptT& res, int64_t act, bool keep) {
   check_linear(x, w, b, res, act);
   ddl::DeviceGuard guard(x.device());
-  auto r = product_forward(x, w, Tensor(), get(b), Tensor(), get(res), (int)act, keep && act != ffn::ACT_NONE, "linear");
-  return {r.first.view(out_sizes(x, w.size(0))), r.second};
+  Kept kept;
+  Tensor y = product_forward(x, w, Tensor(), get(b), Tensor(), get(res), (int)act, keep && act != ffn::ACT_NONE, &kept, "linear");
+  return {y.view(out_sizes(x, w.size(0))), kept.z};
 }
 void check_dy(const Tensor& dy, const Tensor& x, int64_t n, const char* op) {
   check_like(dy, x, op, "the output's gradient");
@@ -317,7 +341,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& dy, const Tenso
     BAD_UNLESS(zz.is_contiguous() && zz.scalar_type() == at::kFloat && zz.dim() == 3 && zz.size(0) == 1 &&
                    zz.size(1) * x.size(-1) == x.numel() && zz.size(2) == up(w.size(0), 16) &&
                    zz.device() == x.device(), "linear: kept sums of another call");
-  auto r = product_backward(dy, x, w, Tensor(), zz, (int)act, need_dx, need_dw, need_db, "linear");
+  auto r = product_backward(dy, {zz, x, {w, Tensor()}}, x.size(-1), (int)act, need_dx, need_dw, need_db, "linear");
   return {need_dx ? r.dx.view(x.sizes()) : r.dx, r.dw[0], r.db[0]};
 }
 
@@ -342,19 +366,25 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptT& b, const OptT& res, int64_t act) {
     at::AutoDispatchBelowADInplaceOrView below;
     Needs::remember(ctx, {true, true, has(b), has(res)});
-    auto r = linear_forward(x, w, b, res, act, true);
-    ctx->save_for_backward({x, w, std::get<1>(r)});
+    ddl::DeviceGuard guard(x.device());
+    Kept kept;
+    Tensor y = product_forward(x, w, Tensor(), get(b), Tensor(), get(res), (int)act, act != ffn::ACT_NONE, &kept, "linear");
+    ctx->save_for_backward({kept.x, kept.w[0], kept.z});
     ctx->saved_data["act"] = act;
+    ctx->saved_data["width"] = x.size(-1);
     ctx->set_materialize_grads(false);
-    return std::get<0>(r);
+    return y.view(out_sizes(x, w.size(0)));
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_second_derivative("linear");
     if (!grads[0].defined()) return variable_list(5);
     const auto saved = ctx->get_saved_variables();
     const Needs need(ctx);
-    auto r = linear_backward(grads[0], saved[0], saved[1], saved[2], ctx->saved_data["act"].toInt(), need(0), need(1), need(2));
-    return {std::get<0>(r), std::get<1>(r), std::get<2>(r), need(3) ? grads[0] : Tensor(), Tensor()};
+    ddl::DeviceGuard guard(grads[0].device());
+    const int64_t width = ctx->saved_data["width"].toInt();
+    auto r = product_backward(grads[0], {saved[2], saved[0], {saved[1], Tensor()}}, width, (int)ctx->saved_data["act"].toInt(), need(0),
+                              need(1), need(2), "linear");
+    return {need(0) ? r.dx.view(out_sizes(grads[0], width)) : r.dx, r.dw[0], r.db[0], need(3) ? grads[0] : Tensor(), Tensor()};
   }
 };
 Tensor linear(const Tensor& x, const Tensor& w, const OptT& b, const OptT& res, int64_t act) {
@@ -377,8 +407,9 @@ std::tuple<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& wg, cons
                                          int64_t act, bool keep) {
   check_gated(x, wg, wu, bg, bu, act);
   ddl::DeviceGuard guard(x.device());
-  auto r = product_forward(x, wg, wu, get(bg), get(bu), Tensor(), (int)act, keep, "gated_linear");
-  return {r.first.view(out_sizes(x, wg.size(0))), r.second};
+  Kept kept;
+  Tensor h = product_forward(x, wg, wu, get(bg), get(bu), Tensor(), (int)act, keep, &kept, "gated_linear");
+  return {h.view(out_sizes(x, wg.size(0))), kept.z};
 }
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_backward(const Tensor& dy, const Tensor& x, const Tensor& wg,
                                                                   const Tensor& wu, const Tensor& z, int64_t act, bool need_dx,
@@ -389,7 +420,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_backward(const Tensor& 
                  z.size(1) * x.size(-1) == x.numel() && z.size(2) == up(wg.size(0), 16) && z.device() == x.device(),
              "gated_linear: the backward pass needs the sums kept by the forward pass");
   ddl::DeviceGuard guard(x.device());
-  auto r = product_backward(dy, x, wg, wu, z, (int)act, need_dx, need_dw, need_db, "gated_linear");
+  auto r = product_backward(dy, {z, x, {wg, wu}}, x.size(-1), (int)act, need_dx, need_dw, need_db, "gated_linear");
   return {need_dx ? r.dx.view(x.sizes()) : r.dx, r.dw[0], r.dw[1], r.db[0], r.db[1]};
 }
 struct GatedFn : torch::autograd::Function<GatedFn> {
@@ -397,21 +428,27 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
                         int64_t act) {
     at::AutoDispatchBelowADInplaceOrView below;
     Needs::remember(ctx, {true, true, true, has(bg), has(bu)});
-    auto r = gated_forward(x, wg, wu, bg, bu, act, true);
-    ctx->save_for_backward({x, wg, wu, std::get<1>(r)});
+    ddl::DeviceGuard guard(x.device());
+    Kept kept;
+    Tensor h = product_forward(x, wg, wu, get(bg), get(bu), Tensor(), (int)act, true, &kept, "gated_linear");
+    ctx->save_for_backward({kept.x, kept.w[0], kept.w[1], kept.z});
     ctx->saved_data["act"] = act;
+    ctx->saved_data["width"] = x.size(-1);
     ctx->set_materialize_grads(false);
-    return std::get<0>(r);
+    return h.view(out_sizes(x, wg.size(0)));
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_second_derivative("gated_linear");
     if (!grads[0].defined()) return variable_list(6);
     const auto s = ctx->get_saved_variables();
     const Needs need(ctx);
-    auto [dx, dwg, dwu, dbg, dbu] = gated_backward(grads[0], s[0], s[1], s[2], s[3], ctx->saved_data["act"].toInt(), need(0),
-                                                   need(1) || need(2), need(3) || need(4));
+    ddl::DeviceGuard guard(grads[0].device());
+    const int64_t width = ctx->saved_data["width"].toInt();
+    auto r = product_backward(grads[0], {s[3], s[0], {s[1], s[2]}}, width, (int)ctx->saved_data["act"].toInt(), need(0),
+                              need(1) || need(2), need(3) || need(4), "gated_linear");
     auto only = [&](int i, const Tensor& t) { return need(i) ? t : Tensor(); };
-    return {dx, only(1, dwg), only(2, dwu), only(3, dbg), only(4, dbu), Tensor()};
+    return {need(0) ? r.dx.view(out_sizes(grads[0], width)) : r.dx, only(1, r.dw[0]), only(2, r.dw[1]), only(3, r.db[0]),
+            only(4, r.db[1]), Tensor()};
   }
 };
 Tensor gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu, const OptT& bg, const OptT& bu, int64_t act) {

@@ -178,6 +178,7 @@ struct GemmArgs {
   int splits = 1;
   Epilogue ep;
 };
+enum Tile : int { TILE_128x32 = 0, TILE_64x64 = 1, TILE_128x128 = 2, TILE_256x128 = 3, TILE_256x256 = 4, N_TILES = 5 };
 // bytes of `partial` the launch needs with the split it would choose (0: none)
 struct GemmPlan { int cfg = 0, splits = 1; long ldw = 0; long partial_floats = 0; };
 GemmPlan gemm_plan(int dtype, const GemmArgs& a);
@@ -215,6 +216,7 @@ struct ActBwdArgs {
   bool dual = false;
   int M = 0, N = 0;
   float* part = nullptr;                  // [chunks][1 + dual][N] column sums of dz, null: none
+  void* db[2] = {nullptr, nullptr};       // instead, with one chunk: the column sums themselves, in the element type
   int chunks = 0;
 };
 int act_bwd_chunks(int dtype, int M, int N);

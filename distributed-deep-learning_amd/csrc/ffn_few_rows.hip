@@ -13,7 +13,7 @@ namespace ddl {
 namespace ffn {
 namespace {
 
-constexpr int NW = 8, U = 4;
+constexpr int NW = 8, U = 8;
 
 template <typename T, bool VEC>
 __device__ __forceinline__ typename Mma<T>::Frag load_chunk(const T* row, int k, int K) {

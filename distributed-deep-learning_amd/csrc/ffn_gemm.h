@@ -3,9 +3,10 @@
 //
 //   out[m][n] = epilogue( sum_k P(n, k) Q(m, k) )
 //
-// P sits on the A side of the MFMA and Q on the B side, so that a lane's accumulators are 16 CONSECUTIVE outputs of one row
-// (rows n of a wave are dealt to the MFMA's A rows as n = 16 (i / 4) + 4 t + i % 4 for tile t): bias, residual and result move
-// as 16-byte vectors without a detour through LDS.
+// P sits on the A side of the MFMA and Q on the B side, so that a lane's accumulators are consecutive outputs of one row, 16 bytes of
+// them, and four lanes hold 64 bytes: 16 bits: rows n of a wave are dealt to the MFMA's A rows as n = 32 (t / 2) + 8 (i / 4) +
+// 4 (t % 2) + i % 4 for tile t, so that a pair of tiles gives eight values; fp32: n = 16 t + i, four values a tile.  Bias, residual
+// and result move as such vectors without a detour through LDS.
 //
 // Tiles: LDS holds a 128-byte wide k slab (64 values of 16 bits, 32 of fp32) of both operands, filled by direct
 // global -> LDS loads of 16 bytes a lane, double buffered: slab t+1 is in flight while slab t is multiplied.  A lane whose
@@ -41,8 +42,8 @@ template <typename T> __device__ __forceinline__ typename Mma<T>::Frag read_tran
 }
 
 // ---- one operand's staging and reading -----------------------------------------------------------------------------
-// R: rows of the tile; G: how the wave's tiles are dealt to rows (see `row_of`); SIDE_P: the A side
-template <typename T, int R, int THREADS, bool KC, bool SIDE_P, bool DUAL, int G>
+// R: rows of the tile; SIDE_P: the A side
+template <typename T, int R, int THREADS, bool KC, bool SIDE_P, bool DUAL>
 struct Operand {
   static constexpr int ES = sizeof(T), EPC = 16 / ES, TK = 128 / ES;
   static constexpr int CPR = KC ? 8 : R * ES / 16;         // 16-byte chunks per LDS row
@@ -51,20 +52,18 @@ struct Operand {
   static_assert(ROUNDS >= 1 && R * 8 % THREADS == 0, "tile / workgroup size");
   static constexpr bool F32 = ES == 4;
 
+  // bits of the LDS row that differ between the lanes of one read place the 16-byte chunks
   static __device__ __forceinline__ int swizzle(int row) {
-    if (KC) {
-      if (SIDE_P) return DUAL ? (row & 3) | ((row >> 3) & 1) << 2 : (row & 3) | ((row >> 4) & 1) << 2;
-      return F32 && G > 1 ? (row / G) & 7 : row & 7;
-    }
-    if (F32) return 0;                                     // 16 lanes read 256 contiguous bytes of one k
-    if (SIDE_P) return ((row & 1) | ((row >> 1) & 1) << 3) & (CPR - 1);
+    if (KC) return SIDE_P && !F32 ? (row & 3) | ((row >> 3) & 1) << 2 : row & 7;
+    if (F32) return 0;                                     // 16 lanes read 64 contiguous bytes of one k
+    if (SIDE_P) return ((row & 3) << 2) & (CPR - 1);
     return ((row & 3) << 1 | ((row >> 3) & 1) << 3) & (CPR - 1);
   }
 
   // Rounds r, r + CLS, ... of a thread lie a constant distance apart: their swizzles agree.  So it carries CLS pointers.
   static constexpr int STEP_ROWS = THREADS / CPR;          // LDS rows from one round to the next
-  static constexpr int CLS = KC && SIDE_P && STEP_ROWS < 32 ? 2 : 1;
-  static_assert(ROUNDS == 1 || STEP_ROWS >= (KC ? (SIDE_P ? 16 : 8 * G) : F32 ? 1 : SIDE_P ? 4 : 16), "rounds swizzle differently");
+  static constexpr int CLS = KC && STEP_ROWS < 16 ? 2 : 1;
+  static_assert(ROUNDS == 1 || STEP_ROWS >= (KC ? (SIDE_P && !F32 ? 16 : 8) : F32 ? 1 : SIDE_P ? 4 : 16), "rounds swizzle differently");
   const char* ptr[CLS];
   int kpos[CLS];                                           // k inside a slab of round 0 (1) of the class
   long stride, step;                                       // bytes between rounds of a class; between slabs
@@ -122,15 +121,19 @@ struct Operand {
     }
     advance(step);
   }
+  // the same where nothing lies outside
+  __device__ __forceinline__ void stage_inside(char* lds) {
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) stage_round(lds, r);
+    advance(step);
+  }
 
   // rows of the operand that lane index i (0..15) of tile t stands for, inside a wave's rows starting at w0
   static __device__ __forceinline__ int row_of(int w0, int t, int i) {
     if (SIDE_P) {
-      if (DUAL) return (t >= 2 ? R / 2 : 0) + w0 + 8 * (i >> 2) + 4 * (t & 1) + (i & 3);
-      if (F32 && !KC) return w0 + 4 * i + t;
-      return w0 + 16 * (i >> 2) + 4 * t + (i & 3);
+      if (DUAL && t >= 2) { w0 += R / 2; t -= 2; }
+      return F32 ? w0 + 16 * t + i : w0 + 32 * (t >> 1) + 8 * (i >> 2) + 4 * (t & 1) + (i & 3);
     }
-    if (F32) return w0 + 16 * G * (t / G) + G * i + t % G;
     return w0 + 16 * t + i;
   }
 
@@ -141,33 +144,22 @@ struct Operand {
     if constexpr (KC) {
       const int row = row_of(w0, t, i);
       return *reinterpret_cast<const Frag*>(lds + row * 128 + (((s * 4 + kg) ^ swizzle(row)) * 16));
+    } else if constexpr (F32) {
+      Frag f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = reinterpret_cast<const float*>(lds + (s * 16 + kg * 4 + e) * (R * 4))[row_of(w0, t, i)];
+      return f;
     } else {
-      static_assert(!F32, "fp32 tiles are read in groups");
       // columns of this lane's 8 bytes: four consecutive rows of the operand
-      const int q = i >> 2, pp = i & 3, col = SIDE_P ? w0 + 16 * pp + 4 * t : w0 + 16 * t + 4 * pp;
+      const int q = i >> 2, pp = i & 3, col = SIDE_P ? w0 + 32 * (t >> 1) + 8 * pp + 4 * (t & 1) : w0 + 16 * t + 4 * pp;
       const int k0 = s * 32 + kg * 8 + q, k1 = k0 + 4;
       return read_transposed<T>(lds + k0 * (R * 2) + ((col / 8) ^ swizzle(k0)) * 16 + (col & 4) * 2,
                                 lds + k1 * (R * 2) + ((col / 8) ^ swizzle(k1)) * 16 + (col & 4) * 2);
     }
   }
   template <int NT> static __device__ __forceinline__ void read(const char* lds, int w0, int s, Frag (&f)[NT]) {
-    if constexpr (F32 && !KC) {
-      // one 16-byte read per k covers four tiles (G = 4) or one 8-byte read two (G = 2)
-      const int l = threadIdx.x & 63, i = l & 15, kg = l >> 4;
 #pragma unroll
-      for (int t = 0; t < NT; t += G) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int k = s * 16 + kg * 4 + e;
-          const float* p = reinterpret_cast<const float*>(lds + k * (R * 4)) + row_of(w0, t, i);
-#pragma unroll
-          for (int j = 0; j < G; ++j) f[t + j][e] = p[j];
-        }
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) f[t] = read_one(lds, w0, s, t);
-    }
+    for (int t = 0; t < NT; ++t) f[t] = read_one(lds, w0, s, t);
   }
 };
 
@@ -183,62 +175,69 @@ __device__ __forceinline__ void tile_of(int id, int tn, int tm, int& nt, int& mt
   nt = in / gm;
 }
 
-// Results of a wave: lane holds rows 4 kg + r of each MFMA tile (16 or 2 x 8 consecutive columns of the output), column i (a row of
-// the output).  n: first column; aligned: it is a multiple of 8.
+// Results of a wave: lane holds rows 4 kg + r of each MFMA tile, i.e. V consecutive columns of the output for every tile (fp32) or pair
+// of tiles (16 bits), and column i (a row of the output).  Dual products: the upper half of the tiles belongs to the second weight.
 template <typename T, typename P, typename Q, bool PKC, bool QKC, bool DUAL, int NT, int MT>
 __device__ __forceinline__ void finish(const GemmArgs& a, const f32x4 (&acc)[NT][MT], int n0, int pw0, int m0, int qw0, int which,
                                        int split) {
-  const int l = threadIdx.x & 63, i = l & 15, kg = l >> 4;
-  const int n = n0 + pw0 + (DUAL ? 8 : 16) * kg;
-  const bool aligned = (n0 & 7) == 0;
   constexpr bool PLAIN = !(PKC && QKC);                    // gradients take neither bias nor activation
-  constexpr int V = DUAL ? 8 : 16;
-  float b0[V], b1[V];
-  if (!PLAIN && a.partial == nullptr) {
-    load_bias<T, V>(a.ep, 0, n, a.N, aligned, b0);
-    if (DUAL) load_bias<T, V>(a.ep, 1, n, a.N, aligned, b1);
-  }
+  constexpr int V = 16 / sizeof(T), TPV = V / 4, PARTS = (DUAL ? NT / 2 : NT) / TPV;
+  const int l = threadIdx.x & 63, i = l & 15, kg = l >> 4;
+  const int n1 = n0 + pw0 + V * kg;                        // part p: columns n1 + 4 V p ..
+  const bool aligned = n0 % V == 0;
 #pragma unroll
-  for (int u = 0; u < MT; ++u) {
-    const int m = m0 + Q::row_of(qw0, u, i);
-    if (m >= a.M) continue;
-    float v[16];
+  for (int p = 0; p < PARTS; ++p) {
+    const int n = n1 + 4 * V * p;
+    float b0[V], b1[V];
+    if (!PLAIN && a.partial == nullptr) {
+      load_bias<T, V>(a.ep, 0, n, a.N, aligned, b0);
+      if (DUAL) load_bias<T, V>(a.ep, 1, n, a.N, aligned, b1);
+    }
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int u = 0; u < MT; ++u) {
+      const int m = m0 + Q::row_of(qw0, u, i);
+      if (m >= a.M) continue;
+      float v[V], w[V];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[(sizeof(T) == 4 && !PKC) ? 4 * r + t : 4 * t + r] = acc[t][u][r];
-    if (a.partial != nullptr) {                            // rows of whole vectors: ldw is N rounded up to 16
-      float* d = a.partial + (((long)split * (a.nout * (DUAL ? 2 : 1)) + which) * a.M + m) * a.ldw + n;
-      store_some<float, V>(d, v, a.N - n, aligned && n < a.N);
-      if (DUAL) store_some<float, V>(d + a.M * a.ldw, v + 8, a.N - n, aligned && n < a.N);
-    } else {
-      epilogue_store<T, DUAL, PLAIN, V>(a.ep, which, m, n, a.N, aligned, v, v + (DUAL ? 8 : 0), b0, b1);
+      for (int e = 0; e < V; ++e) {
+        v[e] = acc[p * TPV + e / 4][u][e % 4];
+        w[e] = DUAL ? acc[(DUAL ? NT / 2 : 0) + p * TPV + e / 4][u][e % 4] : 0.f;
+      }
+      if (a.partial != nullptr) {                          // rows of whole vectors: ldw is N rounded up to 16
+        float* d = a.partial + (((long)split * (a.nout * (DUAL ? 2 : 1)) + which) * a.M + m) * a.ldw + n;
+        store_some<float, V>(d, v, a.N - n, aligned && n < a.N);
+        if (DUAL) store_some<float, V>(d + a.M * a.ldw, w, a.N - n, aligned && n < a.N);
+      } else {
+        epilogue_store<T, DUAL, PLAIN, V>(a.ep, which, m, n, a.N, aligned, v, w, b0, b1);
+      }
     }
   }
 }
 
-// this wave's LDS reads and loads are done; behind the barrier so are the others'
-__device__ __forceinline__ void meet() {
+// this wave's LDS reads are done, and all but its last N loads; behind the barrier so are the others'
+template <int N> __device__ __forceinline__ void meet() {
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0070);                      // vmcnt(0) lgkmcnt(0)
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
 
-// ---- tiles of any size, with their edges: latency and ragged shapes -------------------------------------------------------
-// Double buffered slabs of 128 bytes of k; slab t + 1 is in flight while slab t is multiplied.
-template <typename T, int BN, int BM, int WN, int WM, bool PKC, bool QKC, bool DUAL>
+// ---- tiles of any size, with their edges: small and fp32 products -----------------------------------------------------------
+// A ring of RING slabs of 128 bytes of k; while one is multiplied, the next RING - 1 are in flight.  One barrier a slab: behind it
+// slab t has landed for everyone, and everyone is done with slab t - 1, whose buffer is filled anew.  Small tiles have long
+// rings: with one wave a SIMD nothing else covers a load's two microseconds from memory.
+template <typename T, int BN, int BM, int WN, int WM, int RING, bool PKC, bool QKC, bool DUAL>
 __global__ void __launch_bounds__(WN * WM * 64) gemm_kernel(GemmArgs a) {
   constexpr int THREADS = WN * WM * 64;
   constexpr int NT = BN / WN / 16, MT = BM / WM / 16;
   static_assert(NT == 4, "a wave covers 64 rows of P");
   static_assert(!DUAL || PKC, "dual products: k-contiguous weights");
-  constexpr int G = sizeof(T) == 4 ? (MT >= 4 ? 4 : MT) : 1;
   constexpr int TN = DUAL ? BN / 2 : BN;                   // output columns of a tile
-  using P = Operand<T, BN, THREADS, PKC, true, DUAL, 4>;
-  using Q = Operand<T, BM, THREADS, QKC, false, false, G>;
-  constexpr int TK = P::TK, SLAB = P::BYTES + Q::BYTES;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * SLAB];
+  using P = Operand<T, BN, THREADS, PKC, true, DUAL>;
+  using Q = Operand<T, BM, THREADS, QKC, false, false>;
+  constexpr int TK = P::TK, SLAB = P::BYTES + Q::BYTES, LOADS = P::ROUNDS + Q::ROUNDS;
+  static_assert((RING - 2) * LOADS <= 63, "loads in flight beyond the counter");
+  __shared__ __attribute__((aligned(1024))) char lds[RING * SLAB];
 
   const int tm1 = (a.M + BM - 1) / BM;
   int nt, mt;
@@ -259,66 +258,84 @@ __global__ void __launch_bounds__(WN * WM * 64) gemm_kernel(GemmArgs a) {
 
   P pop;
   Q qop;
-  auto issue = [&](int slab, int buf) {
-    const int seg = slab / slabs, ks = slab - seg * slabs;
-    if (slab == s_begin || ks == 0) {
-      pop.init((const T*)a.p[seg], a.ldp[seg], (const T*)a.p[1], a.ldp[1], n0, a.N, ks * TK);
-      qop.init((const T*)a.q[seg + which], a.ldq[seg + which], nullptr, 0, m0, a.M, ks * TK);
+  int seg = s_begin < s_end ? s_begin / slabs : 0, ks = s_begin - seg * slabs, fill = 0;     // of the slab issued next
+  const bool inside = n0 + TN <= a.N && m0 + BM <= a.M;
+  auto seek = [&]() {
+    pop.init((const T*)a.p[seg], a.ldp[seg], (const T*)a.p[1], a.ldp[1], n0, a.N, ks * TK);
+    qop.init((const T*)a.q[seg + which], a.ldq[seg + which], nullptr, 0, m0, a.M, ks * TK);
+  };
+  auto issue = [&]() {
+    if (ks == slabs) {
+      ks = 0;
+      ++seg;
+      seek();
     }
-    pop.stage(lds + buf * SLAB, a.K - ks * TK);
-    qop.stage(lds + buf * SLAB + P::BYTES, a.K - ks * TK);
+    if (inside && (ks + 1) * TK <= a.K) {
+      pop.stage_inside(lds + fill * SLAB);
+      qop.stage_inside(lds + fill * SLAB + P::BYTES);
+    } else {
+      pop.stage(lds + fill * SLAB, a.K - ks * TK);
+      qop.stage(lds + fill * SLAB + P::BYTES, a.K - ks * TK);
+    }
+    ++ks;
+    fill = fill + 1 == RING ? 0 : fill + 1;
   };
   if (s_begin < s_end) {
-    issue(s_begin, 0);
+    seek();
+    for (int i = 0; i < RING - 1 && s_begin + i < s_end; ++i) issue();
+    int at = 0;
     for (int slab = s_begin; slab < s_end; ++slab) {
-      const int buf = (slab - s_begin) & 1;
-      if (slab + 1 < s_end) {
-        issue(slab + 1, buf ^ 1);
-        __builtin_amdgcn_s_waitcnt(0xF70 | ((P::ROUNDS + Q::ROUNDS) & 15));    // vmcnt: slab's loads have landed
-      } else {
-        __builtin_amdgcn_s_waitcnt(0xF70);
-      }
+      // loads still in flight behind slab's own: RING - 2 slabs, none at the end
+      constexpr int AHEAD = (RING - 2) * LOADS;
+      asm volatile("" ::: "memory");
+      if (slab + RING - 2 < s_end) __builtin_amdgcn_s_waitcnt(0x0F70 | (AHEAD & 15) | (AHEAD >> 4) << 14);
+      else __builtin_amdgcn_s_waitcnt(0x0F70);
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
+      if (slab + RING - 1 < s_end) issue();
+      const char* ps = lds + at * SLAB;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         typename P::Frag pf[NT];
         typename Q::Frag qf[MT];
-        P::template read<NT>(lds + buf * SLAB, pw0, s, pf);
-        Q::template read<MT>(lds + buf * SLAB + P::BYTES, qw0, s, qf);
+        P::template read<NT>(ps, pw0, s, pf);
+        Q::template read<MT>(ps + P::BYTES, qw0, s, qf);
 #pragma unroll
         for (int u = 0; u < MT; ++u)
 #pragma unroll
           for (int t = 0; t < NT; ++t) acc[t][u] = Mma<T>::mma(pf[t], qf[u], acc[t][u]);
       }
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_barrier();                        // everyone has read this slab: it may be overwritten
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this wave has read the slab before it meets the others
+      at = at + 1 == RING ? 0 : at + 1;
     }
   }
   finish<T, P, Q, PKC, QKC, DUAL, NT, MT>(a, acc, n0, pw0, m0, qw0, which, split);
 }
 
-// ---- 256 x 256 tiles of 16-bit operands -------------------------------------------------------------------------------------
+// ---- large products of 16-bit operands ----------------------------------------------------------------------------------------
 // Bound by the matrix cores; what keeps them from their rate is everything that is not a product between two barriers.  So the
 // loop over slabs is one block of straight-line code with ONE barrier, in which the LDS reads and the loads are dealt out between
 // the products:
 //   half 0's products   beside   the LDS reads of half 1
 //   -- all waves have read this slab, and the next one has landed --
-//   half 1's products   beside   the LDS reads of the next slab's half 0 and the loads of the slab after it
+//   half 1's products   beside   the LDS reads of the next slab's half 0 and the loads of the slab RING later
 // P's registers are double, Q's mostly single: a Q tile is replaced right behind its last product.  The last two tiles are double
 // too, so that the reads end before the products do and the wait in front of the barrier finds them done.
 // No edges in the loop: the slab with the end of k comes first (the order of a sum is free), and a tile that would reach beyond the
 // output is moved back inside (it computes some results a second time; both writers hold the same bits).  So N and M are at
 // least a tile.  The second contraction segment has the first one's strides and is reached by a jump.
-template <typename T, bool PKC, bool QKC, bool DUAL>
-__global__ void __launch_bounds__(512) gemm_big_kernel(GemmArgs a) {
-  constexpr int BN = 256, BM = 256, THREADS = 512, WN = 4, NT = 4, MT = 8, DBL = 2, SNG = MT - DBL;
+template <typename T, int BN, int BM, int WN, int WM, int RING, bool PKC, bool QKC, bool DUAL>
+__global__ void __launch_bounds__(WN * WM * 64) gemm_big_kernel(GemmArgs a) {
+  constexpr int THREADS = WN * WM * 64, NT = 4, MT = BM / WM / 16, DBL = 2, SNG = MT - DBL;
+  static_assert(BN / WN == 64, "a wave covers 64 rows of P");
   constexpr int TN = DUAL ? BN / 2 : BN, EPC = 16 / sizeof(T);
-  using P = Operand<T, BN, THREADS, PKC, true, DUAL, 4>;
-  using Q = Operand<T, BM, THREADS, QKC, false, false, 1>;
+  using P = Operand<T, BN, THREADS, PKC, true, DUAL>;
+  using Q = Operand<T, BM, THREADS, QKC, false, false>;
   constexpr int TK = P::TK, SLAB = P::BYTES + Q::BYTES;
-  static_assert(P::ROUNDS == 4 && Q::ROUNDS == 4 && P::CLS == 1 && Q::CLS == 1, "one load of the slab per row of products");
-  __shared__ __attribute__((aligned(1024))) char lds[2 * SLAB];
+  constexpr int LOADS = P::ROUNDS + Q::ROUNDS;             // loads of a slab, dealt out over the rows of products
+  static_assert(NT <= MT && P::CLS == 1 && Q::CLS == 1, "dealing of reads and loads");
+  __shared__ __attribute__((aligned(1024))) char lds[RING * SLAB];
+  static_assert(RING >= 2 && (RING - 2) * LOADS <= 63, "loads in flight beyond the counter");
 
   const int tm1 = (a.M + BM - 1) / BM;
   int nt, mt;
@@ -334,7 +351,7 @@ __global__ void __launch_bounds__(512) gemm_big_kernel(GemmArgs a) {
   const int full = a.K / TK, tails = a.K % TK ? a.nseg : 0, all = tails + full * a.nseg;
   const int per = (all + a.splits - 1) / a.splits, s_begin = split * per, s_end = min(all, s_begin + per);
   const int wave = threadIdx.x >> 6, wn = wave % WN, wm = wave / WN;
-  const int pw0 = DUAL ? wn * 32 : wn * 64, qw0 = wm * (BM / 2);
+  const int pw0 = DUAL ? wn * 32 : wn * 64, qw0 = wm * (BM / WM);
 
   f32x4 acc[NT][MT];
 #pragma unroll
@@ -358,12 +375,12 @@ __global__ void __launch_bounds__(512) gemm_big_kernel(GemmArgs a) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t][u] = Mma<T>::mma(pf[s][t], q, acc[t][u]);
   };
-  // half s's products of the slab in buffer `buf`; NEXT: read the following half (of this slab, or of the other buffer's);
+  // half s's products of the slab in buffer `buf`; NEXT: read the following half (of this slab, or of the next buffer's);
   // LOAD: fill this buffer anew
   auto phase = [&](auto half, auto with_next, auto with_load, int buf) {
     constexpr int s = decltype(half)::value;
     constexpr bool NEXT = decltype(with_next)::value, LOAD = decltype(with_load)::value;
-    const char* next = lds + (s == 0 ? buf : buf ^ 1) * SLAB;
+    const char* next = lds + (s == 0 ? buf : buf + 1 == RING ? 0 : buf + 1) * SLAB;
     char* load = lds + buf * SLAB;
 #pragma unroll
     for (int u = 0; u < MT; ++u) {
@@ -372,8 +389,11 @@ __global__ void __launch_bounds__(512) gemm_big_kernel(GemmArgs a) {
         if (u < DBL) q2[s ^ 1][u] = Q::read_one(next + P::BYTES, qw0, s ^ 1, SNG + u);
       }
       if constexpr (LOAD) {
-        if (u < 4) pop.stage_round(load, u);
-        else qop.stage_round(load + P::BYTES, u - 4);
+#pragma unroll
+        for (int r = u * LOADS / MT; r < (u + 1) * LOADS / MT; ++r) {
+          if (r < P::ROUNDS) pop.stage_round(load, r);
+          else qop.stage_round(load + P::BYTES, r - P::ROUNDS);
+        }
       }
       products(s, u);
       if constexpr (NEXT) {
@@ -388,64 +408,66 @@ __global__ void __launch_bounds__(512) gemm_big_kernel(GemmArgs a) {
   constexpr std::false_type NO{};
   const int count = s_end - s_begin;
   if (count > 0) {
-    int left = seek(s_begin);
-    pop.stage(lds, left);
-    qop.stage(lds + P::BYTES, left);
-    if (count > 1) {
-      left = seek(s_begin + 1);
-      pop.stage(lds + SLAB, left);
-      qop.stage(lds + SLAB + P::BYTES, left);
+    for (int i = 0; i < RING && i < count; ++i) {
+      const int left = seek(s_begin + i);
+      pop.stage(lds + i * SLAB, left);
+      qop.stage(lds + i * SLAB + P::BYTES, left);
     }
-    meet();
+    meet<0>();
     P::template read<NT>(lds, pw0, 0, pf[0]);
 #pragma unroll
     for (int u = 0; u < SNG; ++u) q1[u] = Q::read_one(lds + P::BYTES, qw0, 0, u);
 #pragma unroll
     for (int u = 0; u < DBL; ++u) q2[0][u] = Q::read_one(lds + P::BYTES, qw0, 0, SNG + u);
     int buf = 0;
-    if (count > 2) {
-      seek(s_begin + 2);
+    if (count > RING) {
+      seek(s_begin + RING);
       // slabs until the jump to the second segment (0: none), and its distance from where the first one ends
-      int to_jump = a.nseg == 2 ? tails + full - (s_begin + 2) : 0;
+      int to_jump = a.nseg == 2 ? tails + full - (s_begin + RING) : 0;
       const long p_jump = a.nseg == 2 ? (const char*)a.p[1] - (const char*)a.p[0] - full * pop.step : 0;
       const long q_jump = a.nseg == 2 ? (const char*)a.q[1] - (const char*)a.q[0] - full * qop.step : 0;
-      for (int i = 0; i < count - 2; ++i) {
+      for (int i = 0; i < count - RING; ++i) {
         phase(H0, YES, NO, buf);
-        meet();
+        meet<(RING - 2) * LOADS>();                        // the next slab has landed; later ones stay in flight
         phase(H1, YES, YES, buf);
         const bool jump = --to_jump == 0;
         pop.advance(pop.step + (jump ? p_jump : 0));
         qop.advance(qop.step + (jump ? q_jump : 0));
-        buf ^= 1;
+        buf = buf + 1 == RING ? 0 : buf + 1;
       }
     }
-    phase(H0, YES, NO, buf);
-    if (count > 1) {
-      meet();
-      phase(H1, YES, NO, buf);
-      buf ^= 1;
+    for (int i = min(count, RING) - 1; i > 0; --i) {
       phase(H0, YES, NO, buf);
+      meet<0>();
+      phase(H1, YES, NO, buf);
+      buf = buf + 1 == RING ? 0 : buf + 1;
     }
+    phase(H0, YES, NO, buf);
     phase(H1, NO, NO, buf);
   }
   finish<T, P, Q, PKC, QKC, DUAL, NT, MT>(a, acc, n0, pw0, m0, qw0, which, split);
 }
 
-template <typename T, int BN, int BM, int WN, int WM> void run_cfg(const GemmArgs& a, hipStream_t s) {
+template <typename T, int BN, int BM, int WN, int WM, int RING> void run_cfg(const GemmArgs& a, hipStream_t s) {
   const long tn = (a.N + (a.dual ? BN / 2 : BN) - 1) / (a.dual ? BN / 2 : BN), tm = (long)((a.M + BM - 1) / BM) * a.nout;
   const dim3 grid((unsigned)(tn * tm), (unsigned)a.splits), block(WN * WM * 64);
-  if (a.dual) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, true, true, true>), grid, block, 0, s, a);
-  else if (a.p_kc) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, true, true, false>), grid, block, 0, s, a);
-  else if (a.q_kc) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, false, true, false>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, false, false, false>), grid, block, 0, s, a);
+  if (a.dual) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, RING, true, true, true>), grid, block, 0, s, a);
+  else if (a.p_kc) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, RING, true, true, false>), grid, block, 0, s, a);
+  else if (a.q_kc) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, RING, false, true, false>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, RING, false, false, false>), grid, block, 0, s, a);
 }
-template <typename T> void run_big(const GemmArgs& a, hipStream_t s) {
-  const int tn = a.dual ? 128 : 256;
-  const dim3 grid((unsigned)((long)((a.N + tn - 1) / tn) * ((a.M + 255) / 256) * a.nout), (unsigned)a.splits), block(512);
-  if (a.dual) hipLaunchKernelGGL((gemm_big_kernel<T, true, true, true>), grid, block, 0, s, a);
-  else if (a.p_kc) hipLaunchKernelGGL((gemm_big_kernel<T, true, true, false>), grid, block, 0, s, a);
-  else if (a.q_kc) hipLaunchKernelGGL((gemm_big_kernel<T, false, true, false>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((gemm_big_kernel<T, false, false, false>), grid, block, 0, s, a);
+template <typename T, int BN, int BM, int WN, int WM, int RING> void run_big(const GemmArgs& a, hipStream_t s) {
+  const int tn = a.dual ? BN / 2 : BN;
+  const dim3 grid((unsigned)((long)((a.N + tn - 1) / tn) * ((a.M + BM - 1) / BM) * a.nout), (unsigned)a.splits), block(WN * WM * 64);
+  if (a.dual) hipLaunchKernelGGL((gemm_big_kernel<T, BN, BM, WN, WM, RING, true, true, true>), grid, block, 0, s, a);
+  else if (a.p_kc) hipLaunchKernelGGL((gemm_big_kernel<T, BN, BM, WN, WM, RING, true, true, false>), grid, block, 0, s, a);
+  else if (a.q_kc) hipLaunchKernelGGL((gemm_big_kernel<T, BN, BM, WN, WM, RING, false, true, false>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((gemm_big_kernel<T, BN, BM, WN, WM, RING, false, false, false>), grid, block, 0, s, a);
+}
+template <typename T> void run_small(const GemmArgs& a, int cfg, hipStream_t s) {
+  if (cfg == TILE_128x32) run_cfg<T, 128, 32, 2, 2, 4>(a, s);
+  else if (cfg == TILE_64x64) run_cfg<T, 64, 64, 1, 4, 4>(a, s);
+  else run_cfg<T, 128, 128, 2, 2, 2>(a, s);
 }
 }  // namespace
 }  // namespace ffn

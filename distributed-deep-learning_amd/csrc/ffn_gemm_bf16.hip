@@ -4,9 +4,9 @@
 namespace ddl {
 namespace ffn {
 void launch_gemm_bf16(const GemmArgs& a, int cfg, hipStream_t s) {
-  if (cfg == 0) run_cfg<__bf16, 128, 32, 2, 1>(a, s);
-  else if (cfg == 1) run_cfg<__bf16, 128, 128, 2, 2>(a, s);
-  else run_big<__bf16>(a, s);
+  if (cfg == TILE_256x256) run_big<__bf16, 256, 256, 4, 2, 2>(a, s);
+  else if (cfg == TILE_256x128) run_big<__bf16, 256, 128, 4, 2, 3>(a, s);
+  else run_small<__bf16>(a, cfg, s);
 }
 }  // namespace ffn
 }  // namespace ddl

@@ -4,9 +4,6 @@
 
 namespace ddl {
 namespace ffn {
-void launch_gemm_f32(const GemmArgs& a, int cfg, hipStream_t s) {
-  if (cfg == 0) run_cfg<float, 128, 32, 2, 1>(a, s);
-  else run_cfg<float, 128, 128, 2, 2>(a, s);
-}
+void launch_gemm_f32(const GemmArgs& a, int cfg, hipStream_t s) { run_small<float>(a, cfg, s); }
 }  // namespace ffn
 }  // namespace ddl

@@ -23,35 +23,47 @@ __global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ src, lo
   }
 }
 
-// ---- join: the splits' sums in split order, then the product's epilogue -------------------------------------------------
+// ---- join: the splits' sums, then the product's epilogue -----------------------------------------------------------------
+// Four groups of threads take every fourth split each and meet in LDS in a fixed order: with up to 32 splits of few rows one thread
+// an output would wait for memory 32 times.
 template <typename T, bool DUAL>
 __global__ void __launch_bounds__(256) join_kernel(GemmArgs a) {
-  constexpr int V = 4;
-  const int per = (int)(a.ldw / V), planes = a.nout * (DUAL ? 2 : 1);
-  const long rows = (long)a.M * a.nout, total = rows * per, plane = (long)a.M * a.ldw;
-  for (long i = blockIdx.x * 256L + threadIdx.x; i < total; i += gridDim.x * 256L) {
-    const long row = i / per;
-    const int n = (int)(i - row * per) * V, which = (int)(row / a.M);
-    const long m = row - (long)which * a.M;
-    if (n >= a.N) continue;
+  constexpr int V = 4, GROUPS = 4, TX = 64, D = DUAL ? 2 : 1;
+  __shared__ float red[GROUPS - 1][TX][D * V + 1];
+  const int per = (int)(a.ldw / V), planes = a.nout * D, tx = threadIdx.x % TX, g = threadIdx.x / TX;
+  const long rows = (long)a.M * a.nout, total = rows * per, plane = (long)a.M * a.ldw, step = planes * plane;
+  const long i = blockIdx.x * (long)TX + tx, row = i / per;
+  const int n = (int)(i - row * per) * V, which = (int)(row / a.M);
+  const long m = row - (long)which * a.M;
+  const bool in = i < total && n < a.N;
+  float v[D * V];
+#pragma unroll
+  for (int e = 0; e < D * V; ++e) v[e] = 0.f;
+  if (in) {
     const float* p = a.partial + which * plane + m * a.ldw + n;
-    float v[V] = {0.f, 0.f, 0.f, 0.f}, w[V] = {0.f, 0.f, 0.f, 0.f}, b0[V], b1[V];
-    for (int s = 0; s < a.splits; ++s) {
-      float t[V];
-      load_vec<float, V>(p, t);
+#pragma unroll 4
+    for (int s = g; s < a.splits; s += GROUPS) {
+      float t[D * V];
+      load_vec<float, V>(p + s * step, t);
+      if (DUAL) load_vec<float, V>(p + s * step + plane, t + (D - 1) * V);
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[e] += t[e];
-      if (DUAL) {
-        load_vec<float, V>(p + plane, t);
-#pragma unroll
-        for (int e = 0; e < V; ++e) w[e] += t[e];
-      }
-      p += planes * plane;
+      for (int e = 0; e < D * V; ++e) v[e] += t[e];
     }
-    load_bias<T, V>(a.ep, 0, n, a.N, true, b0);
-    load_bias<T, V>(a.ep, 1, n, a.N, true, b1);
-    epilogue_store<T, DUAL, false, V>(a.ep, which, m, n, a.N, true, v, w, b0, b1);
   }
+  if (g > 0) {
+#pragma unroll
+    for (int e = 0; e < D * V; ++e) red[g - 1][tx][e] = v[e];
+  }
+  __syncthreads();
+  if (g > 0 || !in) return;
+#pragma unroll
+  for (int q = 0; q < GROUPS - 1; ++q)
+#pragma unroll
+    for (int e = 0; e < D * V; ++e) v[e] += red[q][tx][e];
+  float b0[V], b1[V];
+  load_bias<T, V>(a.ep, 0, n, a.N, true, b0);
+  load_bias<T, V>(a.ep, 1, n, a.N, true, b1);
+  epilogue_store<T, DUAL, false, V>(a.ep, which, m, n, a.N, true, v, v + (D - 1) * V, b0, b1);
 }
 
 // ---- backward of the activation -----------------------------------------------------------------------------------------
@@ -104,7 +116,7 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(ActBwdArgs a) {
       }
     }
   }
-  if (a.part == nullptr) return;                           // uniform over the grid
+  if (a.part == nullptr && a.db[0] == nullptr) return;      // uniform over the grid
 #pragma unroll
   for (int d = 0; d < D; ++d) {
     __syncthreads();
@@ -117,7 +129,8 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(ActBwdArgs a) {
       float s = 0.f;
 #pragma unroll
       for (int y = 0; y < TY; ++y) s += red[y][c];
-      a.part[((long)blockIdx.y * D + d) * a.N + col] = s;
+      if (a.db[0] != nullptr) ((T*)a.db[d])[col] = from_f<T>(s);
+      else a.part[((long)blockIdx.y * D + d) * a.N + col] = s;
     }
   }
 }
@@ -165,13 +178,15 @@ void launch_pack(int dtype, const void* src, long s_row, long s_col, void* dst, 
 void launch_join(int dtype, const float* partial, const GemmArgs& a0, hipStream_t s) {
   GemmArgs a = a0;
   a.partial = const_cast<float*>(partial);
-  const dim3 grid(grid_for((long)a.M * a.nout * (a.ldw / 4)));
+  const dim3 grid((unsigned)(((long)a.M * a.nout * (a.ldw / 4) + 63) / 64));
   if (a.dual) DDL_BY_TYPE(dtype, hipLaunchKernelGGL((join_kernel<T, true>), grid, dim3(256), 0, s, a));
   else DDL_BY_TYPE(dtype, hipLaunchKernelGGL((join_kernel<T, false>), grid, dim3(256), 0, s, a));
 }
 
-// rows are dealt to so many workgroups that the grid holds about 2048 of them, eight rows at least each
+// Rows are dealt to so many workgroups that the grid holds about 2048 of them, eight rows at least each.  Up to 64 rows are one
+// chunk: eight turns of a thread cost less than the second launch (a step over 30 x 4096 fp32: 4 + 2.4 us as two).
 int act_bwd_chunks(int dtype, int M, int N) {
+  if (M <= 64) return 1;
   const int cols = 32 * 16 / esize(dtype), nb = (N + cols - 1) / cols;
   int c = 2048 / (nb < 1 ? 1 : nb);
   const int most = (M + 7) / 8;
@@ -195,32 +210,49 @@ void launch_colsum(int out_dtype, const float* part, int chunks, int nvec, long 
 }
 
 // ---- choice of tile and split -------------------------------------------------------------------------------------------
+// The estimate in microseconds that picks both: a launch, then the fullest CU's workgroups.  `one` / `two`: what 128 bytes of k of one
+// workgroup alone / of two side by side on a CU cost, `end`: a tile's epilogue.  Measured with graphs of 20 calls, bf16:
+//   512 x 1024 x 4096:   64 x 64 tiles 11.4 us, 128 x 128 16.6;        gated: 22 us against 18.4
+//   1500 x 5000 x 5000:  256 x 128 88 us, 256 x 256 122, 128 x 128 100
+//   128 x 4096 x 512:    64 x 64 in 16 splits 9.6 us, in 1: 28
+// A split writes its sums in fp32 and a second launch joins them: 3 us and the bytes at 2 TB/s.
+namespace {
+struct TileCost { int bn, bm; double one, two, end; };
+constexpr TileCost COST16[N_TILES] = {{128, 32, .35, .45, .5}, {64, 64, .39, .48, .5}, {128, 128, .80, 1.40, 1.}, {256, 128, 1.05, 2.1, 2.5},
+                                      {256, 256, 1.7, 3.4, 5.}};
+constexpr TileCost COST32[N_TILES] = {{128, 32, .75, 1.1, .5}, {64, 64, .80, 1.22, .5}, {128, 128, 2.4, 4.6, 1.}, {}, {}};
+}  // namespace
+
 GemmPlan gemm_plan(int dtype, const GemmArgs& a) {
-  auto tiles = [&](int bn, int bm) {
-    const long w = a.dual ? bn / 2 : bn;
-    return ((a.N + w - 1) / w) * (long)((a.M + bm - 1) / bm) * a.nout;
-  };
-  GemmPlan p;
-  p.ldw = (a.N + 15) / 16 * 16;
-  const bool same = a.nseg == 1 || (a.ldp[0] == a.ldp[1] && a.ldq[0] == a.ldq[1]);
-  const bool holds = a.M >= 256 && a.N >= (a.dual ? 128 : 256) && same;
-  if (dtype != F32 && holds && tiles(256, 256) >= 192) p.cfg = 2;
-  else if (a.M > 64) p.cfg = 1;
-  else p.cfg = 0;
-  const long t = p.cfg == 2 ? tiles(256, 256) : p.cfg == 1 ? tiles(128, 128) : tiles(128, 32);
+  GemmPlan best;
+  best.ldw = (a.N + 15) / 16 * 16;
   const int tk = 128 / esize(dtype);
   const long slabs = (long)((a.K + tk - 1) / tk) * a.nseg;
-  const long want = p.cfg == 2 ? 1 : (p.cfg == 1 ? 384 : 1024) / (t < 1 ? 1 : t);
-  long s = want;
-  if (s > slabs / 4) s = slabs / 4;
-  if (s > 32) s = 32;
-  p.splits = s < 2 ? 1 : (int)s;
-  if (p.splits > 1) {                                      // no empty splits
-    const long per = (slabs + p.splits - 1) / p.splits;
-    p.splits = (int)((slabs + per - 1) / per);
-    p.partial_floats = (long)p.splits * a.nout * (a.dual ? 2 : 1) * a.M * p.ldw;
+  const bool same = a.nseg == 1 || (a.ldp[0] == a.ldp[1] && a.ldq[0] == a.ldq[1]);
+  double best_us = 1e300;
+  for (int cfg = 0; cfg < N_TILES; ++cfg) {
+    const TileCost& c = (dtype == F32 ? COST32 : COST16)[cfg];
+    const int width = a.dual ? c.bn / 2 : c.bn;
+    if (c.bn == 0 || (cfg >= TILE_256x128 && !(same && a.N >= width && a.M >= c.bm))) continue;     // tiles without edges
+    // k-strided operands give a narrow tile only a part of a memory line's neighbours per request
+    const double f = cfg <= TILE_64x64 && !(a.p_kc && a.q_kc) ? 1.3 : 1.0;
+    const long tiles = ((a.N + width - 1) / width) * (long)((a.M + c.bm - 1) / c.bm) * a.nout;
+    for (long s = 1; s <= 32; s *= 2) {
+      if (s > 1 && (s > slabs / 2 || tiles * s > 2048)) break;
+      const long per = (slabs + s - 1) / s, splits = slabs > 0 ? (slabs + per - 1) / per : 1;      // no empty splits
+      const long wgs = (tiles * splits + 255) / 256;
+      double us = 3.5 + per * f * ((wgs / 2) * c.two + (wgs % 2) * c.one) + wgs * c.end;
+      const double floats = (double)splits * a.nout * (a.dual ? 2 : 1) * a.M * best.ldw;
+      if (splits > 1) us += 3.0 + floats * 4 / 2e6;
+      if (us < best_us) {
+        best_us = us;
+        best.cfg = cfg;
+        best.splits = (int)splits;
+        best.partial_floats = splits > 1 ? (long)floats : 0;
+      }
+    }
   }
-  return p;
+  return best;
 }
 
 void launch_gemm(int dtype, GemmArgs a, const GemmPlan& plan, hipStream_t s) {

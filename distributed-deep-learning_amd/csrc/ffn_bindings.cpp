@@ -660,6 +660,11 @@ NormGrads norm_backward(const NormIn& in, const Tensor& st, const Tensor& dr, co
     part = at::empty({a.groups, 5, a.C}, in.x.options().dtype(at::kFloat));
     a.part = part.data_ptr<float>();
   }
+  Tensor means;
+  if (any && a.dh != nullptr && ffn::norm_bwd_wants_means(a.C)) {
+    means = at::empty({2, a.M}, in.x.options().dtype(at::kFloat));
+    a.means = means.data_ptr<float>();
+  }
   ffn::launch_norm_bwd(s.dtype, a, cur_stream());
   if (any) ffn::launch_colsum(a.param_f32 ? (int)ffn::F32 : s.dtype, a.part, a.groups, 5, a.C, outs, cur_stream());
   return g;

@@ -35,10 +35,12 @@ struct NormArgs {
   const void *dr = nullptr, *dh = nullptr;                     // either may be null (zero)
   void *dx = nullptr, *dy = nullptr, *dgate = nullptr;         // dgate: full gates only
   float* part = nullptr;                 // [groups][5][C]: dgate, dpost_w, dpost_b, dpre_w, dpre_b
+  float* means = nullptr;                // [2][M], wide rows with `part`: what the rows' pass leaves for the columns' pass
   int groups = 0;
 };
 constexpr int NORM_MAX_C = 16384;
 int norm_bwd_groups(int M, int C);
+bool norm_bwd_wants_means(int C);
 void launch_norm_fwd(int dtype, const NormArgs& a, hipStream_t s);
 void launch_norm_bwd(int dtype, const NormArgs& a, hipStream_t s);
 

@@ -70,7 +70,8 @@ bool is_operand(const Tensor& t) {
   const int64_t epc = 16 / t.element_size();
   return t.numel() == 0 || ((t.size(1) <= 1 || t.stride(1) == 1) && t.size(1) % epc == 0 && rows_aligned(t));
 }
-Operand operand(const Tensor& t, int dtype, int64_t width) {        // t: 2-D [rows, width], or packed already
+// t: 2-D [rows, width], or packed already.  What has to be packed joins `todo`, for one launch.
+Operand operand(const Tensor& t, int64_t width, ffn::PackArgs& todo) {
   Operand o;
   if (t.size(1) != width) {
     o.keep = t;
@@ -86,7 +87,14 @@ Operand operand(const Tensor& t, int dtype, int64_t width) {        // t: 2-D [r
   }
   o.ld = line(t.size(1), t);
   o.keep = at::empty({t.size(0), o.ld}, t.options());
-  ffn::launch_pack(dtype, t.data_ptr(), t.stride(0), t.stride(1), o.keep.data_ptr(), o.ld, t.size(0), (int)t.size(1), cur_stream());
+  ffn::PackItem& it = todo.item[todo.count++];
+  it.src = t.data_ptr();
+  it.dst = o.keep.data_ptr();
+  it.s_row = t.stride(0);
+  it.s_col = t.stride(1);
+  it.ld = o.ld;
+  it.rows = t.size(0);
+  it.cols = (int)t.size(1);
   o.p = o.keep.data_ptr();
   return o;
 }
@@ -188,7 +196,9 @@ Tensor product_forward(const Tensor& x, const Tensor& w0, const Tensor& w1, cons
     ffn::launch_few_rows(dtype, f, cur_stream());
     return out;
   }
-  const Operand xo = operand(x2, dtype, K), wo = operand(w0, dtype, K), vo = dual ? operand(w1, dtype, K) : Operand();
+  ffn::PackArgs todo;
+  const Operand xo = operand(x2, K, todo), wo = operand(w0, K, todo), vo = dual ? operand(w1, K, todo) : Operand();
+  ffn::launch_pack(dtype, todo, cur_stream());
   if (kept != nullptr) {
     if (xo.keep.size(1) != K) kept->x = xo.keep;
     if (wo.keep.size(1) != K) kept->w[0] = wo.keep;
@@ -232,13 +242,20 @@ ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width,
   // dz in padded rows; without an activation dz is dy itself
   const bool make_dz = z.defined() && (need_dx || need_dw);
   Tensor dz;
-  Operand dzo[2];
+  Operand dzo[2], wo[2], xo;
+  ffn::PackArgs todo;
   if (make_dz) {
     dz = at::empty({D, M, line(N, x)}, x.options());
     for (int d = 0; d < D; ++d) dzo[d] = own_operand(dz[d]);
   } else if (need_dx || need_dw) {
-    dzo[0] = operand(dy2, dtype, N);
+    dzo[0] = operand(dy2, N, todo);
   }
+  if (K > 0 && need_dx) {
+    wo[0] = operand(rows_of(w0), K, todo);
+    if (dual) wo[1] = operand(rows_of(w1), K, todo);
+  }
+  if (K > 0 && need_dw) xo = operand(x2, K, todo);
+  ffn::launch_pack(dtype, todo, cur_stream());
   if (make_dz || need_db) {
     ffn::ActBwdArgs b;
     b.dy = dy2.data_ptr();
@@ -271,7 +288,6 @@ ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width,
   }
   if (K == 0) return r;
   if (need_dx) {                                                     // dx[m][k] = sum over weights, n of dz[m][n] w[n][k]
-    const Operand wo[2] = {operand(rows_of(w0), dtype, K), dual ? operand(rows_of(w1), dtype, K) : Operand()};
     ffn::GemmArgs g;
     g.N = K; g.M = M; g.K = N;
     g.nseg = D;
@@ -284,7 +300,6 @@ ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width,
     run_gemm(dtype, g, x);
   }
   if (need_dw) {                                                     // dw[n][k] = sum over m of dz[m][n] x[m][k]
-    const Operand xo = operand(x2, dtype, K);
     ffn::GemmArgs g;
     g.N = K; g.M = N; g.K = M;
     g.nout = D;

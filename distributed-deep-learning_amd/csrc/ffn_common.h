@@ -178,7 +178,7 @@ struct GemmArgs {
   int splits = 1;
   Epilogue ep;
 };
-enum Tile : int { TILE_128x32 = 0, TILE_64x64 = 1, TILE_128x128 = 2, TILE_256x128 = 3, TILE_256x256 = 4, N_TILES = 5 };
+enum Tile : int { TILE_128x32 = 0, TILE_64x32 = 1, TILE_64x64 = 2, TILE_128x128 = 3, TILE_256x128 = 4, TILE_256x256 = 5, N_TILES = 6 };
 // bytes of `partial` the launch needs with the split it would choose (0: none)
 struct GemmPlan { int cfg = 0, splits = 1; long ldw = 0; long partial_floats = 0; };
 GemmPlan gemm_plan(int dtype, const GemmArgs& a);
@@ -200,9 +200,10 @@ constexpr int FEW_ROWS = 32;
 void launch_few_rows(int dtype, const FewRowsArgs& a, hipStream_t s);
 
 // ---- pointwise companions (ffn_pointwise.hip) --------------------------------------------------------------------------
-// dst [rows][ld_dst] = src with arbitrary strides, columns beyond `cols` up to ld_dst zero
-void launch_pack(int dtype, const void* src, long s_row, long s_col, void* dst, long ld_dst, long rows, int cols,
-                 hipStream_t s);
+// dst [rows][ld] = src with any strides, columns from `cols` on zero
+struct PackItem { const void* src = nullptr; void* dst = nullptr; long s_row = 0, s_col = 0, ld = 0, rows = 0; int cols = 0; };
+struct PackArgs { PackItem item[4]; int count = 0; };
+void launch_pack(int dtype, const PackArgs& a, hipStream_t s);
 void launch_join(int dtype, const float* partial, const GemmArgs& a, hipStream_t s);
 struct ActBwdArgs {
   const void* dy = nullptr;

@@ -64,6 +64,7 @@ struct Operand {
   static constexpr int STEP_ROWS = THREADS / CPR;          // LDS rows from one round to the next
   static constexpr int CLS = KC && STEP_ROWS < 16 ? 2 : 1;
   static_assert(ROUNDS == 1 || STEP_ROWS >= (KC ? (SIDE_P && !F32 ? 16 : 8) : F32 ? 1 : SIDE_P ? 4 : 16), "rounds swizzle differently");
+  static_assert(!DUAL || STEP_ROWS <= R / 2, "a round of a dual operand lies in one of its matrices");
   const char* ptr[CLS];
   int kpos[CLS];                                           // k inside a slab of round 0 (1) of the class
   long stride, step;                                       // bytes between rounds of a class; between slabs
@@ -225,10 +226,11 @@ template <int N> __device__ __forceinline__ void meet() {
 // ---- tiles of any size, with their edges: small and fp32 products -----------------------------------------------------------
 // A ring of RING slabs of 128 bytes of k; while one is multiplied, the next RING - 1 are in flight.  One barrier a slab: behind it
 // slab t has landed for everyone, and everyone is done with slab t - 1, whose buffer is filled anew.  Small tiles have long
-// rings: with one wave a SIMD nothing else covers a load's two microseconds from memory.
-template <typename T, int BN, int BM, int WN, int WM, int RING, bool PKC, bool QKC, bool DUAL>
-__global__ void __launch_bounds__(WN * WM * 64) gemm_kernel(GemmArgs a) {
-  constexpr int THREADS = WN * WM * 64;
+// rings: with one wave a SIMD nothing else covers a load's two microseconds from memory.  WK = 2: two groups of waves
+// take one k half of every slab each and add their sums in LDS at the end, where the tile alone has too little work for four SIMDs.
+template <typename T, int BN, int BM, int WN, int WM, int WK, int RING, bool PKC, bool QKC, bool DUAL>
+__global__ void __launch_bounds__(WN * WM * WK * 64) gemm_kernel(GemmArgs a) {
+  constexpr int THREADS = WN * WM * WK * 64;
   constexpr int NT = BN / WN / 16, MT = BM / WM / 16;
   static_assert(NT == 4, "a wave covers 64 rows of P");
   static_assert(!DUAL || PKC, "dual products: k-contiguous weights");
@@ -247,7 +249,7 @@ __global__ void __launch_bounds__(WN * WM * 64) gemm_kernel(GemmArgs a) {
   // contraction: a.nseg segments of `slabs` slabs each; this split takes [s_begin, s_end) of all of them
   const int slabs = (a.K + TK - 1) / TK, all = slabs * a.nseg;
   const int per = (all + a.splits - 1) / a.splits, s_begin = split * per, s_end = min(all, s_begin + per);
-  const int wave = threadIdx.x >> 6, wn = wave % WN, wm = wave / WN;
+  const int wave = threadIdx.x >> 6, wn = wave % WN, wm = wave / WN % WM, wk = wave / (WN * WM);
   const int pw0 = DUAL ? wn * 32 : wn * 64, qw0 = wm * (BM / WM);
 
   f32x4 acc[NT][MT];
@@ -294,20 +296,36 @@ __global__ void __launch_bounds__(WN * WM * 64) gemm_kernel(GemmArgs a) {
       asm volatile("" ::: "memory");
       if (slab + RING - 1 < s_end) issue();
       const char* ps = lds + at * SLAB;
+      constexpr int HALVES = 2 / WK;
+      typename P::Frag pf[HALVES][NT];                     // all reads first: the second half's run beside the first's products
+      typename Q::Frag qf[HALVES][MT];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        typename P::Frag pf[NT];
-        typename Q::Frag qf[MT];
-        P::template read<NT>(ps, pw0, s, pf);
-        Q::template read<MT>(ps + P::BYTES, qw0, s, qf);
-#pragma unroll
-        for (int u = 0; u < MT; ++u)
-#pragma unroll
-          for (int t = 0; t < NT; ++t) acc[t][u] = Mma<T>::mma(pf[t], qf[u], acc[t][u]);
+      for (int s = 0; s < HALVES; ++s) {
+        P::template read<NT>(ps, pw0, WK == 2 ? wk : s, pf[s]);
+        Q::template read<MT>(ps + P::BYTES, qw0, WK == 2 ? wk : s, qf[s]);
       }
+#pragma unroll
+      for (int s = 0; s < HALVES; ++s) mma_tiles<T, NT, MT>(pf[s], qf[s], acc);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this wave has read the slab before it meets the others
       at = at + 1 == RING ? 0 : at + 1;
     }
+  }
+  if constexpr (WK == 2) {
+    f32x4* join = reinterpret_cast<f32x4*>(lds) + (wave % (WN * WM)) * 64 * NT * MT + (threadIdx.x & 63);
+    static_assert(WN * WM * 64 * NT * MT * 16 <= RING * SLAB, "sums of one group of waves");
+    __syncthreads();                                       // the ring has been read
+    if (wk == 1) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < MT; ++u) join[(t * MT + u) * 64] = acc[t][u];
+    }
+    __syncthreads();
+    if (wk == 1) return;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int u = 0; u < MT; ++u) acc[t][u] += join[(t * MT + u) * 64];
   }
   finish<T, P, Q, PKC, QKC, DUAL, NT, MT>(a, acc, n0, pw0, m0, qw0, which, split);
 }
@@ -448,13 +466,13 @@ __global__ void __launch_bounds__(WN * WM * 64) gemm_big_kernel(GemmArgs a) {
   finish<T, P, Q, PKC, QKC, DUAL, NT, MT>(a, acc, n0, pw0, m0, qw0, which, split);
 }
 
-template <typename T, int BN, int BM, int WN, int WM, int RING> void run_cfg(const GemmArgs& a, hipStream_t s) {
+template <typename T, int BN, int BM, int WN, int WM, int WK, int RING> void run_cfg(const GemmArgs& a, hipStream_t s) {
   const long tn = (a.N + (a.dual ? BN / 2 : BN) - 1) / (a.dual ? BN / 2 : BN), tm = (long)((a.M + BM - 1) / BM) * a.nout;
-  const dim3 grid((unsigned)(tn * tm), (unsigned)a.splits), block(WN * WM * 64);
-  if (a.dual) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, RING, true, true, true>), grid, block, 0, s, a);
-  else if (a.p_kc) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, RING, true, true, false>), grid, block, 0, s, a);
-  else if (a.q_kc) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, RING, false, true, false>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, RING, false, false, false>), grid, block, 0, s, a);
+  const dim3 grid((unsigned)(tn * tm), (unsigned)a.splits), block(WN * WM * WK * 64);
+  if (a.dual) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, WK, RING, true, true, true>), grid, block, 0, s, a);
+  else if (a.p_kc) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, WK, RING, true, true, false>), grid, block, 0, s, a);
+  else if (a.q_kc) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, WK, RING, false, true, false>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, WK, RING, false, false, false>), grid, block, 0, s, a);
 }
 template <typename T, int BN, int BM, int WN, int WM, int RING> void run_big(const GemmArgs& a, hipStream_t s) {
   const int tn = a.dual ? BN / 2 : BN;
@@ -465,9 +483,10 @@ template <typename T, int BN, int BM, int WN, int WM, int RING> void run_big(con
   else hipLaunchKernelGGL((gemm_big_kernel<T, BN, BM, WN, WM, RING, false, false, false>), grid, block, 0, s, a);
 }
 template <typename T> void run_small(const GemmArgs& a, int cfg, hipStream_t s) {
-  if (cfg == TILE_128x32) run_cfg<T, 128, 32, 2, 2, 4>(a, s);
-  else if (cfg == TILE_64x64) run_cfg<T, 64, 64, 1, 4, 4>(a, s);
-  else run_cfg<T, 128, 128, 2, 2, 2>(a, s);
+  if (cfg == TILE_128x32) run_cfg<T, 128, 32, 2, 2, 1, 4>(a, s);
+  else if (cfg == TILE_64x32) run_cfg<T, 64, 32, 1, 2, 2, 4>(a, s);
+  else if (cfg == TILE_64x64) run_cfg<T, 64, 64, 1, 4, 1, 4>(a, s);
+  else run_cfg<T, 128, 128, 2, 2, 1, 2>(a, s);
 }
 }  // namespace
 }  // namespace ffn

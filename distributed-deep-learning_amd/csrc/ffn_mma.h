@@ -36,5 +36,25 @@ template <> struct Mma<float> {          // four 16x16x4 products over the four 
   }
 };
 
+// acc += P Q for NT x MT tiles.  fp32: all tiles of one k before the next k, since a product that waits for the one before it on the
+// same accumulator leaves the matrix core idle.
+template <typename T, int NT, int MT>
+__device__ __forceinline__ void mma_tiles(const typename Mma<T>::Frag (&p)[NT], const typename Mma<T>::Frag (&q)[MT],
+                                          f32x4 (&acc)[NT][MT]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int u = 0; u < MT; ++u)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[t][e], q[u][e], acc[t][u], 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int u = 0; u < MT; ++u)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t][u] = Mma<T>::mma(p[t], q[u], acc[t][u]);
+  }
+}
+
 }  // namespace ffn
 }  // namespace ddl

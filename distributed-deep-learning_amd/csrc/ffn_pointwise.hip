@@ -7,19 +7,20 @@ namespace ddl {
 namespace ffn {
 namespace {
 
-// ---- pack: any strides -> rows of 16-byte multiples, padding zero (it enters sums over k) -------------------------------
+// ---- pack: any strides -> rows of 16-byte multiples, padding zero (it enters sums over k); one launch for a product's operands -----
 template <typename T>
-__global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ src, long s_row, long s_col, T* __restrict__ dst,
-                                                   long ld, long rows, int cols) {
+__global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
   constexpr int V = 16 / sizeof(T);
-  const long per = ld / V, total = rows * per;
+  const PackItem& it = a.item[blockIdx.y];
+  const T* src = (const T*)it.src;
+  const long per = it.ld / V, total = it.rows * per;
   for (long i = blockIdx.x * 256L + threadIdx.x; i < total; i += gridDim.x * 256L) {
     const long r = i / per;
     const int c = (int)(i - r * per) * V;
     Pack<T, V> x;
 #pragma unroll
-    for (int e = 0; e < V; ++e) x.v[e] = c + e < cols ? src[r * s_row + (c + e) * s_col] : (T)0.f;
-    *reinterpret_cast<Pack<T, V>*>(dst + r * ld + c) = x;
+    for (int e = 0; e < V; ++e) x.v[e] = c + e < it.cols ? src[r * it.s_row + (c + e) * it.s_col] : (T)0.f;
+    *reinterpret_cast<Pack<T, V>*>((T*)it.dst + r * it.ld + c) = x;
   }
 }
 
@@ -168,11 +169,14 @@ unsigned grid_for(long items) {
     DDL_HIP_CHECK(hipGetLastError());                             \
   } while (0)
 
-void launch_pack(int dtype, const void* src, long s_row, long s_col, void* dst, long ld_dst, long rows, int cols,
-                 hipStream_t s) {
-  if (rows <= 0 || ld_dst <= 0) return;
-  DDL_BY_TYPE(dtype, hipLaunchKernelGGL(pack_kernel<T>, dim3(grid_for(rows * ld_dst * sizeof(T) / 16)), dim3(256), 0, s,
-                                        (const T*)src, s_row, s_col, (T*)dst, ld_dst, rows, cols));
+void launch_pack(int dtype, const PackArgs& a, hipStream_t s) {
+  long most = 0;
+  for (int i = 0; i < a.count; ++i) {
+    const long v = a.item[i].rows * a.item[i].ld * esize(dtype) / 16;
+    most = v > most ? v : most;
+  }
+  if (most == 0) return;
+  DDL_BY_TYPE(dtype, hipLaunchKernelGGL(pack_kernel<T>, dim3(grid_for(most), a.count), dim3(256), 0, s, a));
 }
 
 void launch_join(int dtype, const float* partial, const GemmArgs& a0, hipStream_t s) {
@@ -218,9 +222,9 @@ void launch_colsum(int out_dtype, const float* part, int chunks, int nvec, long 
 // A split writes its sums in fp32 and a second launch joins them: 3 us and the bytes at 2 TB/s.
 namespace {
 struct TileCost { int bn, bm; double one, two, end; };
-constexpr TileCost COST16[N_TILES] = {{128, 32, .35, .45, .5}, {64, 64, .39, .48, .5}, {128, 128, .80, 1.40, 1.}, {256, 128, 1.05, 2.1, 2.5},
-                                      {256, 256, 1.7, 3.4, 5.}};
-constexpr TileCost COST32[N_TILES] = {{128, 32, .75, 1.1, .5}, {64, 64, .80, 1.22, .5}, {128, 128, 2.4, 4.6, 1.}, {}, {}};
+constexpr TileCost COST16[N_TILES] = {{128, 32, .52, .62, .5}, {64, 32, .30, .38, .5}, {64, 64, .39, .48, .5}, {128, 128, .80, 1.40, 1.},
+                                      {256, 128, 1.05, 2.1, 2.5}, {256, 256, 1.7, 3.4, 5.}};
+constexpr TileCost COST32[N_TILES] = {{128, 32, .75, 1.35, .5}, {64, 32, .48, .75, .5}, {64, 64, .77, 1.22, .5}, {128, 128, 2.4, 4.3, 1.}, {}, {}};
 }  // namespace
 
 GemmPlan gemm_plan(int dtype, const GemmArgs& a) {

@@ -51,6 +51,8 @@ struct Operand {
   static constexpr int BYTES = R * 128;
   static_assert(ROUNDS >= 1 && R * 8 % THREADS == 0, "tile / workgroup size");
   static constexpr bool F32 = ES == 4;
+  static_assert((THREADS & (THREADS - 1)) == 0, "groups of threads");
+  static __device__ __forceinline__ int tid() { return (int)threadIdx.x & (THREADS - 1); }     // in the group that stages a slab
 
   // bits of the LDS row that differ between the lanes of one read place the 16-byte chunks
   static __device__ __forceinline__ int swizzle(int row) {
@@ -73,12 +75,12 @@ struct Operand {
   // rows row0 .. of an operand of `rows` rows; b1, ld1: second matrix of a dual operand (rows R/2 ..)
   __device__ __forceinline__ void init(const T* b0, long ld0, const T* b1, long ld1, int row0, int rows, int k0) {
     ok = 0;
-    const int first = threadIdx.x / CPR;
+    const int first = tid() / CPR;
     step = KC ? 128 : (long)TK * ld0 * ES;
     stride = (long)CLS * STEP_ROWS * ld0 * ES;
 #pragma unroll
     for (int r = 0; r < CLS; ++r) {
-      const int lrow = first + r * STEP_ROWS, c = (threadIdx.x % CPR) ^ swizzle(lrow);
+      const int lrow = first + r * STEP_ROWS, c = (tid() % CPR) ^ swizzle(lrow);
       if (KC) {
         kpos[r] = c * EPC;
         ptr[r] = (const char*)(b0 + (long)(row0 + lrow) * ld0 + k0 + kpos[r]);
@@ -102,8 +104,8 @@ struct Operand {
   // round r of a slab that lies inside
   __device__ __forceinline__ void stage_round(char* lds, int r) const {
     const char* src = ptr[r % CLS] + (r / CLS) * stride;
-    if (DUAL && r * STEP_ROWS >= R / 2) src += half + ((int)(threadIdx.x / CPR) + r * STEP_ROWS - R / 2) * lead * ES;
-    load_to_lds(src, lds + (threadIdx.x & ~63) * 16 + r * THREADS * 16);
+    if (DUAL && r * STEP_ROWS >= R / 2) src += half + (tid() / CPR + r * STEP_ROWS - R / 2) * lead * ES;
+    load_to_lds(src, lds + (tid() & ~63) * 16 + r * THREADS * 16);
   }
   __device__ __forceinline__ void advance(long by) {
 #pragma unroll
@@ -111,16 +113,20 @@ struct Operand {
   }
   // the slab at the current position, `left` k remaining, with its edges; moves on
   __device__ __forceinline__ void stage(char* lds, int left) {
-    char* w = lds + (threadIdx.x & ~63) * 16;
+    char* w = lds + (tid() & ~63) * 16;
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
       const char* src = ptr[r % CLS] + (r / CLS) * stride;
-      if (DUAL && r * STEP_ROWS >= R / 2) src += half + ((int)(threadIdx.x / CPR) + r * STEP_ROWS - R / 2) * lead * ES;
+      if (DUAL && r * STEP_ROWS >= R / 2) src += half + (tid() / CPR + r * STEP_ROWS - R / 2) * lead * ES;
       const int k = KC ? kpos[r % CLS] : kpos[0] + r * STEP_ROWS;
       if (!((ok >> r) & 1) || k >= left) src = (const char*)g_zeros;
       load_to_lds(src, w + r * THREADS * 16);
     }
     advance(step);
+  }
+  static __device__ __forceinline__ void stage_zeros(char* lds) {
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) load_to_lds((const char*)g_zeros, lds + (tid() & ~63) * 16 + r * THREADS * 16);
   }
   // the same where nothing lies outside
   __device__ __forceinline__ void stage_inside(char* lds) {
@@ -224,13 +230,14 @@ template <int N> __device__ __forceinline__ void meet() {
 }
 
 // ---- tiles of any size, with their edges: small and fp32 products -----------------------------------------------------------
-// A ring of RING slabs of 128 bytes of k; while one is multiplied, the next RING - 1 are in flight.  One barrier a slab: behind it
-// slab t has landed for everyone, and everyone is done with slab t - 1, whose buffer is filled anew.  Small tiles have long
-// rings: with one wave a SIMD nothing else covers a load's two microseconds from memory.  WK = 2: two groups of waves
-// take one k half of every slab each and add their sums in LDS at the end, where the tile alone has too little work for four SIMDs.
-template <typename T, int BN, int BM, int WN, int WM, int WK, int RING, bool PKC, bool QKC, bool DUAL>
-__global__ void __launch_bounds__(WN * WM * WK * 64) gemm_kernel(GemmArgs a) {
-  constexpr int THREADS = WN * WM * WK * 64;
+// A ring of slabs of 128 bytes of k; while some are multiplied, the next ones are in flight.  One barrier a turn: behind it the
+// turn's slabs have landed for everyone, and everyone is done with the previous turn's, whose buffers are filled anew.
+// Small tiles give a CU too little to do: a wave alone on its SIMD stands still in front of every barrier, LDS read and load.  So more
+// waves share a tile along k: WK = 2 groups take one k half of a slab each, and with GROUPS = 2 a turn has two slabs, each staged
+// and multiplied by a group of its own.  Their sums meet in LDS at the end, in a fixed order.
+template <typename T, int BN, int BM, int WN, int WM, int WK, int GROUPS, int RING, bool PKC, bool QKC, bool DUAL>
+__global__ void __launch_bounds__(WN * WM * WK * GROUPS * 64) gemm_kernel(GemmArgs a) {
+  constexpr int WAVES = WN * WM, THREADS = WAVES * WK * 64, SETS = WK * GROUPS;
   constexpr int NT = BN / WN / 16, MT = BM / WM / 16;
   static_assert(NT == 4, "a wave covers 64 rows of P");
   static_assert(!DUAL || PKC, "dual products: k-contiguous weights");
@@ -238,18 +245,21 @@ __global__ void __launch_bounds__(WN * WM * WK * 64) gemm_kernel(GemmArgs a) {
   using P = Operand<T, BN, THREADS, PKC, true, DUAL>;
   using Q = Operand<T, BM, THREADS, QKC, false, false>;
   constexpr int TK = P::TK, SLAB = P::BYTES + Q::BYTES, LOADS = P::ROUNDS + Q::ROUNDS;
-  static_assert((RING - 2) * LOADS <= 63, "loads in flight beyond the counter");
-  __shared__ __attribute__((aligned(1024))) char lds[RING * SLAB];
+  constexpr int AHEAD = (RING - 2) * LOADS;                // a wave's loads behind the turn's own
+  static_assert(RING >= 2 && AHEAD <= 63, "loads in flight beyond the counter");
+  __shared__ __attribute__((aligned(1024))) char lds[RING * GROUPS * SLAB];
 
   const int tm1 = (a.M + BM - 1) / BM;
   int nt, mt;
   tile_of(blockIdx.x, (a.N + TN - 1) / TN, tm1 * a.nout, nt, mt);
   const int which = mt / tm1, m0 = (mt - which * tm1) * BM, n0 = nt * TN, split = blockIdx.y;
 
-  // contraction: a.nseg segments of `slabs` slabs each; this split takes [s_begin, s_end) of all of them
+  // contraction: a.nseg segments of `slabs` slabs each; this split takes [s_begin, s_end) of all of them, GROUPS a turn
   const int slabs = (a.K + TK - 1) / TK, all = slabs * a.nseg;
   const int per = (all + a.splits - 1) / a.splits, s_begin = split * per, s_end = min(all, s_begin + per);
-  const int wave = threadIdx.x >> 6, wn = wave % WN, wm = wave / WN % WM, wk = wave / (WN * WM);
+  const int turns = (s_end - s_begin + GROUPS - 1) / GROUPS;         // no work: 0 or less
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wm = wave / WN % WM;
+  const int set = wave / WAVES, wk = set % WK, group = set / WK;
   const int pw0 = DUAL ? wn * 32 : wn * 64, qw0 = wm * (BM / WM);
 
   f32x4 acc[NT][MT];
@@ -260,72 +270,76 @@ __global__ void __launch_bounds__(WN * WM * WK * 64) gemm_kernel(GemmArgs a) {
 
   P pop;
   Q qop;
-  int seg = s_begin < s_end ? s_begin / slabs : 0, ks = s_begin - seg * slabs, fill = 0;     // of the slab issued next
   const bool inside = n0 + TN <= a.N && m0 + BM <= a.M;
-  auto seek = [&]() {
-    pop.init((const T*)a.p[seg], a.ldp[seg], (const T*)a.p[1], a.ldp[1], n0, a.N, ks * TK);
-    qop.init((const T*)a.q[seg + which], a.ldq[seg + which], nullptr, 0, m0, a.M, ks * TK);
-  };
+  int next = s_begin + group, seg = -1, fill = 0;          // this group's slab issued next, the segment its pointers are in
   auto issue = [&]() {
-    if (ks == slabs) {
-      ks = 0;
-      ++seg;
-      seek();
+    char* at = lds + (fill * GROUPS + group) * SLAB;
+    if (next < s_end) {
+      const int sg = next / slabs, left = a.K - (next - sg * slabs) * TK;
+      if (sg != seg) {
+        seg = sg;
+        pop.init((const T*)a.p[seg], a.ldp[seg], (const T*)a.p[1], a.ldp[1], n0, a.N, a.K - left);
+        qop.init((const T*)a.q[seg + which], a.ldq[seg + which], nullptr, 0, m0, a.M, a.K - left);
+      }
+      if (inside && left >= TK) {
+        pop.stage_inside(at);
+        qop.stage_inside(at + P::BYTES);
+      } else {
+        pop.stage(at, left);
+        qop.stage(at + P::BYTES, left);
+      }
+      if (GROUPS > 1) {                                    // the other groups' slabs
+        pop.advance((GROUPS - 1) * pop.step);
+        qop.advance((GROUPS - 1) * qop.step);
+      }
+    } else {                                               // a turn that is not full: zeros
+      P::stage_zeros(at);
+      Q::stage_zeros(at + P::BYTES);
     }
-    if (inside && (ks + 1) * TK <= a.K) {
-      pop.stage_inside(lds + fill * SLAB);
-      qop.stage_inside(lds + fill * SLAB + P::BYTES);
-    } else {
-      pop.stage(lds + fill * SLAB, a.K - ks * TK);
-      qop.stage(lds + fill * SLAB + P::BYTES, a.K - ks * TK);
-    }
-    ++ks;
+    next += GROUPS;
     fill = fill + 1 == RING ? 0 : fill + 1;
   };
-  if (s_begin < s_end) {
-    seek();
-    for (int i = 0; i < RING - 1 && s_begin + i < s_end; ++i) issue();
-    int at = 0;
-    for (int slab = s_begin; slab < s_end; ++slab) {
-      // loads still in flight behind slab's own: RING - 2 slabs, none at the end
-      constexpr int AHEAD = (RING - 2) * LOADS;
-      asm volatile("" ::: "memory");
-      if (slab + RING - 2 < s_end) __builtin_amdgcn_s_waitcnt(0x0F70 | (AHEAD & 15) | (AHEAD >> 4) << 14);
-      else __builtin_amdgcn_s_waitcnt(0x0F70);
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      if (slab + RING - 1 < s_end) issue();
-      const char* ps = lds + at * SLAB;
-      constexpr int HALVES = 2 / WK;
-      typename P::Frag pf[HALVES][NT];                     // all reads first: the second half's run beside the first's products
-      typename Q::Frag qf[HALVES][MT];
+  for (int i = 0; i < RING - 1 && i < turns; ++i) issue();
+  int at = 0;
+  for (int turn = 0; turn < turns; ++turn) {
+    asm volatile("" ::: "memory");
+    if (turn + RING - 2 < turns) __builtin_amdgcn_s_waitcnt(0x0F70 | (AHEAD & 15) | (AHEAD >> 4) << 14);
+    else __builtin_amdgcn_s_waitcnt(0x0F70);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (turn + RING - 1 < turns) issue();
+    const char* ps = lds + (at * GROUPS + group) * SLAB;
+    constexpr int HALVES = 2 / WK;
+    typename P::Frag pf[HALVES][NT];                       // all reads first: the second half's run beside the first's products
+    typename Q::Frag qf[HALVES][MT];
 #pragma unroll
-      for (int s = 0; s < HALVES; ++s) {
-        P::template read<NT>(ps, pw0, WK == 2 ? wk : s, pf[s]);
-        Q::template read<MT>(ps + P::BYTES, qw0, WK == 2 ? wk : s, qf[s]);
-      }
-#pragma unroll
-      for (int s = 0; s < HALVES; ++s) mma_tiles<T, NT, MT>(pf[s], qf[s], acc);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this wave has read the slab before it meets the others
-      at = at + 1 == RING ? 0 : at + 1;
+    for (int s = 0; s < HALVES; ++s) {
+      P::template read<NT>(ps, pw0, WK == 2 ? wk : s, pf[s]);
+      Q::template read<MT>(ps + P::BYTES, qw0, WK == 2 ? wk : s, qf[s]);
     }
+#pragma unroll
+    for (int s = 0; s < HALVES; ++s) mma_tiles<T, NT, MT>(pf[s], qf[s], acc);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // this wave has read its slab before it meets the others
+    at = at + 1 == RING ? 0 : at + 1;
   }
-  if constexpr (WK == 2) {
-    f32x4* join = reinterpret_cast<f32x4*>(lds) + (wave % (WN * WM)) * 64 * NT * MT + (threadIdx.x & 63);
-    static_assert(WN * WM * 64 * NT * MT * 16 <= RING * SLAB, "sums of one group of waves");
+  if constexpr (SETS > 1) {
+    static_assert((SETS - 1) * WAVES * 64 * NT * MT * 16 <= RING * GROUPS * SLAB, "sums of the other waves");
+    f32x4* join = reinterpret_cast<f32x4*>(lds) + (wave % WAVES) * 64 * NT * MT + (threadIdx.x & 63);
     __syncthreads();                                       // the ring has been read
-    if (wk == 1) {
+    if (set > 0) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int u = 0; u < MT; ++u) join[(t * MT + u) * 64] = acc[t][u];
+        for (int u = 0; u < MT; ++u) join[(set - 1) * WAVES * 64 * NT * MT + (t * MT + u) * 64] = acc[t][u];
     }
     __syncthreads();
-    if (wk == 1) return;
+    if (set > 0) return;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int i = 0; i < SETS - 1; ++i)
 #pragma unroll
-      for (int u = 0; u < MT; ++u) acc[t][u] += join[(t * MT + u) * 64];
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < MT; ++u) acc[t][u] += join[i * WAVES * 64 * NT * MT + (t * MT + u) * 64];
   }
   finish<T, P, Q, PKC, QKC, DUAL, NT, MT>(a, acc, n0, pw0, m0, qw0, which, split);
 }
@@ -466,13 +480,13 @@ __global__ void __launch_bounds__(WN * WM * 64) gemm_big_kernel(GemmArgs a) {
   finish<T, P, Q, PKC, QKC, DUAL, NT, MT>(a, acc, n0, pw0, m0, qw0, which, split);
 }
 
-template <typename T, int BN, int BM, int WN, int WM, int WK, int RING> void run_cfg(const GemmArgs& a, hipStream_t s) {
+template <typename T, int BN, int BM, int WN, int WM, int WK, int GROUPS, int RING> void run_cfg(const GemmArgs& a, hipStream_t s) {
   const long tn = (a.N + (a.dual ? BN / 2 : BN) - 1) / (a.dual ? BN / 2 : BN), tm = (long)((a.M + BM - 1) / BM) * a.nout;
-  const dim3 grid((unsigned)(tn * tm), (unsigned)a.splits), block(WN * WM * WK * 64);
-  if (a.dual) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, WK, RING, true, true, true>), grid, block, 0, s, a);
-  else if (a.p_kc) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, WK, RING, true, true, false>), grid, block, 0, s, a);
-  else if (a.q_kc) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, WK, RING, false, true, false>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, WK, RING, false, false, false>), grid, block, 0, s, a);
+  const dim3 grid((unsigned)(tn * tm), (unsigned)a.splits), block(WN * WM * WK * GROUPS * 64);
+  if (a.dual) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, WK, GROUPS, RING, true, true, true>), grid, block, 0, s, a);
+  else if (a.p_kc) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, WK, GROUPS, RING, true, true, false>), grid, block, 0, s, a);
+  else if (a.q_kc) hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, WK, GROUPS, RING, false, true, false>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((gemm_kernel<T, BN, BM, WN, WM, WK, GROUPS, RING, false, false, false>), grid, block, 0, s, a);
 }
 template <typename T, int BN, int BM, int WN, int WM, int RING> void run_big(const GemmArgs& a, hipStream_t s) {
   const int tn = a.dual ? BN / 2 : BN;
@@ -483,10 +497,10 @@ template <typename T, int BN, int BM, int WN, int WM, int RING> void run_big(con
   else hipLaunchKernelGGL((gemm_big_kernel<T, BN, BM, WN, WM, RING, false, false, false>), grid, block, 0, s, a);
 }
 template <typename T> void run_small(const GemmArgs& a, int cfg, hipStream_t s) {
-  if (cfg == TILE_128x32) run_cfg<T, 128, 32, 2, 2, 1, 4>(a, s);
-  else if (cfg == TILE_64x32) run_cfg<T, 64, 32, 1, 2, 2, 4>(a, s);
-  else if (cfg == TILE_64x64) run_cfg<T, 64, 64, 1, 4, 1, 4>(a, s);
-  else run_cfg<T, 128, 128, 2, 2, 1, 2>(a, s);
+  if (cfg == TILE_128x32) run_cfg<T, 128, 32, 2, 2, 1, 2, 2>(a, s);
+  else if (cfg == TILE_64x32) run_cfg<T, 64, 32, 1, 2, 2, 2, 3>(a, s);
+  else if (cfg == TILE_64x64) run_cfg<T, 64, 64, 1, 4, 1, 2, 2>(a, s);
+  else run_cfg<T, 128, 128, 2, 2, 1, 1, 2>(a, s);
 }
 }  // namespace
 }  // namespace ffn

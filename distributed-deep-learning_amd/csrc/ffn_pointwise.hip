@@ -187,10 +187,11 @@ void launch_join(int dtype, const float* partial, const GemmArgs& a0, hipStream_
   else DDL_BY_TYPE(dtype, hipLaunchKernelGGL((join_kernel<T, false>), grid, dim3(256), 0, s, a));
 }
 
-// Rows are dealt to so many workgroups that the grid holds about 2048 of them, eight rows at least each.  Up to 64 rows are one
-// chunk: eight turns of a thread cost less than the second launch (a step over 30 x 4096 fp32: 4 + 2.4 us as two).
+// Rows are dealt to so many workgroups that the grid holds about 2048 of them, eight rows at least each.  Up to 32 rows are one
+// chunk: four turns of a thread cost less than the second launch (a step over 30 x 4096 fp32: 4 + 2.4 us as two); the eight turns of
+// 64 x 4096 bf16 cost 16 us.
 int act_bwd_chunks(int dtype, int M, int N) {
-  if (M <= 64) return 1;
+  if (M <= 32) return 1;
   const int cols = 32 * 16 / esize(dtype), nb = (N + cols - 1) / cols;
   int c = 2048 / (nb < 1 ? 1 : nb);
   const int most = (M + 7) / 8;
@@ -215,16 +216,18 @@ void launch_colsum(int out_dtype, const float* part, int chunks, int nvec, long 
 
 // ---- choice of tile and split -------------------------------------------------------------------------------------------
 // The estimate in microseconds that picks both: a launch, then the fullest CU's workgroups.  `one` / `two`: what 128 bytes of k of one
-// workgroup alone / of two side by side on a CU cost, `end`: a tile's epilogue.  Measured with graphs of 20 calls, bf16:
-//   512 x 1024 x 4096:   64 x 64 tiles 11.4 us, 128 x 128 16.6;        gated: 22 us against 18.4
-//   1500 x 5000 x 5000:  256 x 128 88 us, 256 x 256 122, 128 x 128 100
-//   128 x 4096 x 512:    64 x 64 in 16 splits 9.6 us, in 1: 28
+// workgroup alone / of two side by side on a CU cost, `end`: a tile's epilogue.  Fitted to graphs of 20 calls of every tile and split
+// over twelve shapes from 40 x 256 x 512 to 1024 x 2048 x 2048 (rows x columns x k); its choice was 1.3% behind the best of them on
+// the geometric mean, and these are some of the sides, bf16:
+//   256 x 4096 x 1024:   64 x 64 tiles 8.3 us, 128 x 32 9.3, 128 x 128 17.4;     its d_x: 128 x 32 in 4 splits 14.1, 64 x 32 in 2 15.7
+//   512 x 1024 x 1024:   64 x 32 7.5 us, 64 x 64 8.1, 128 x 32 8.7, 64 x 64 in 2 splits 11.2;     its d_w: 128 x 32 6.3, 64 x 32 7.9
+//   1500 x 5000 x 5000:  256 x 128 88 us, 256 x 256 122, 128 x 128 100;          8192 x 8192 x 8192: 256 x 256 first
 // A split writes its sums in fp32 and a second launch joins them: 3 us and the bytes at 2 TB/s.
 namespace {
 struct TileCost { int bn, bm; double one, two, end; };
-constexpr TileCost COST16[N_TILES] = {{128, 32, .52, .62, .5}, {64, 32, .30, .38, .5}, {64, 64, .39, .48, .5}, {128, 128, .80, 1.40, 1.},
+constexpr TileCost COST16[N_TILES] = {{128, 32, .30, .56, .4}, {64, 32, .22, .40, .5}, {64, 64, .30, .53, .4}, {128, 128, .80, 1.40, 1.},
                                       {256, 128, 1.05, 2.1, 2.5}, {256, 256, 1.7, 3.4, 5.}};
-constexpr TileCost COST32[N_TILES] = {{128, 32, .75, 1.35, .5}, {64, 32, .48, .75, .5}, {64, 64, .77, 1.22, .5}, {128, 128, 2.4, 4.3, 1.}, {}, {}};
+constexpr TileCost COST32[N_TILES] = {{128, 32, .71, 1.35, .6}, {64, 32, .42, .75, .6}, {64, 64, .66, 1.23, .7}, {128, 128, 2.4, 3.9, 2.}, {}, {}};
 }  // namespace
 
 GemmPlan gemm_plan(int dtype, const GemmArgs& a) {
@@ -238,14 +241,15 @@ GemmPlan gemm_plan(int dtype, const GemmArgs& a) {
     const TileCost& c = (dtype == F32 ? COST32 : COST16)[cfg];
     const int width = a.dual ? c.bn / 2 : c.bn;
     if (c.bn == 0 || (cfg >= TILE_256x128 && !(same && a.N >= width && a.M >= c.bm))) continue;     // tiles without edges
-    // k-strided operands give a narrow tile only a part of a memory line's neighbours per request
-    const double f = cfg <= TILE_64x64 && !(a.p_kc && a.q_kc) ? 1.3 : 1.0;
+    // k-strided 16-bit operands of 64 columns: every read of LDS is a transposing one, half as wide
+    const double f = dtype != F32 && cfg == TILE_64x64 && !(a.p_kc && a.q_kc) ? 1.2 : 1.0;
     const long tiles = ((a.N + width - 1) / width) * (long)((a.M + c.bm - 1) / c.bm) * a.nout;
     for (long s = 1; s <= 32; s *= 2) {
       if (s > 1 && (s > slabs / 2 || tiles * s > 2048)) break;
       const long per = (slabs + s - 1) / s, splits = slabs > 0 ? (slabs + per - 1) / per : 1;      // no empty splits
       const long wgs = (tiles * splits + 255) / 256;
-      double us = 3.5 + per * f * ((wgs / 2) * c.two + (wgs % 2) * c.one) + wgs * c.end;
+      const double turns = cfg <= TILE_64x64 ? (per + 1) / 2 * 2 : per;     // slabs in pairs
+      double us = 3.5 + turns * f * ((wgs / 2) * c.two + (wgs % 2) * c.one) + wgs * c.end;
       const double floats = (double)splits * a.nout * (a.dual ? 2 : 1) * a.M * best.ldw;
       if (splits > 1) us += 3.0 + floats * 4 / 2e6;
       if (us < best_us) {

@@ -5,6 +5,7 @@
 // where it is stored.
 #pragma once
 #include <hip/hip_runtime.h>
+#include <cfloat>
 #include <cmath>
 #include <cstdint>
 
@@ -173,6 +174,7 @@ struct GemmArgs {
   int N = 0, M = 0, K = 0;                // K: contraction length of ONE segment
   int nseg = 1, nout = 1;
   bool p_kc = true, q_kc = true, dual = false;
+  bool halves = false;                    // outputs m and m + M / 2 are one output's sums: joined (M / 2 rows of out)
   float* partial = nullptr;               // split contraction: [splits][nout * (1 + dual)][M][ldw] sums instead of out
   long ldw = 0;
   int splits = 1;
@@ -213,6 +215,7 @@ struct ActBwdArgs {
   long ldz = 0;
   void* dz[2] = {nullptr, nullptr};       // padded rows; may be null where only the column sums are wanted
   long ldd = 0;
+  bool two = false;                       // dz in two parts: rounded, and what that lacks in rows M ..
   int act = ACT_NONE;
   bool dual = false;
   int M = 0, N = 0;

@@ -184,38 +184,67 @@ __device__ __forceinline__ void tile_of(int id, int tn, int tm, int& nt, int& mt
 
 // Results of a wave: lane holds rows 4 kg + r of each MFMA tile, i.e. V consecutive columns of the output for every tile (fp32) or pair
 // of tiles (16 bits), and column i (a row of the output).  Dual products: the upper half of the tiles belongs to the second weight.
-template <typename T, typename P, typename Q, bool PKC, bool QKC, bool DUAL, int NT, int MT>
+// CHUNK > 0: the sums go through LDS, CHUNK of the wave's row tiles at a time, so that one piece of code serves them in a loop: unrolled over
+// all of them with the activations inside, it outgrows the instruction cache, and a tile waits for its code (8192 x 4096 x 4096 bf16 with
+// gelu and residual: 285 us unrolled, 252 so).  The ring is no longer read then; `lds` is this wave's part, and each lane reads back what it wrote.
+template <typename T, typename P, typename Q, bool PKC, bool QKC, bool DUAL, int NT, int MT, int CHUNK>
 __device__ __forceinline__ void finish(const GemmArgs& a, const f32x4 (&acc)[NT][MT], int n0, int pw0, int m0, int qw0, int which,
-                                       int split) {
+                                       int split, char* lds) {
   constexpr bool PLAIN = !(PKC && QKC);                    // gradients take neither bias nor activation
   constexpr int V = 16 / sizeof(T), TPV = V / 4, PARTS = (DUAL ? NT / 2 : NT) / TPV;
   const int l = threadIdx.x & 63, i = l & 15, kg = l >> 4;
   const int n1 = n0 + pw0 + V * kg;                        // part p: columns n1 + 4 V p ..
   const bool aligned = n0 % V == 0;
+  float b0[PARTS][V], b1[PARTS][V];
+  if (!PLAIN && a.partial == nullptr) {
 #pragma unroll
-  for (int p = 0; p < PARTS; ++p) {
-    const int n = n1 + 4 * V * p;
-    float b0[V], b1[V];
-    if (!PLAIN && a.partial == nullptr) {
-      load_bias<T, V>(a.ep, 0, n, a.N, aligned, b0);
-      if (DUAL) load_bias<T, V>(a.ep, 1, n, a.N, aligned, b1);
+    for (int p = 0; p < PARTS; ++p) {
+      load_bias<T, V>(a.ep, 0, n1 + 4 * V * p, a.N, aligned, b0[p]);
+      if (DUAL) load_bias<T, V>(a.ep, 1, n1 + 4 * V * p, a.N, aligned, b1[p]);
     }
+  }
+  // the sums of row m
+  auto row = [&](int m, const f32x4 (&sums)[NT]) {
+    if (m >= a.M) return;
 #pragma unroll
-    for (int u = 0; u < MT; ++u) {
-      const int m = m0 + Q::row_of(qw0, u, i);
-      if (m >= a.M) continue;
+    for (int p = 0; p < PARTS; ++p) {
+      const int n = n1 + 4 * V * p;
       float v[V], w[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        v[e] = acc[p * TPV + e / 4][u][e % 4];
-        w[e] = DUAL ? acc[(DUAL ? NT / 2 : 0) + p * TPV + e / 4][u][e % 4] : 0.f;
+        v[e] = sums[p * TPV + e / 4][e % 4];
+        w[e] = DUAL ? sums[(DUAL ? NT / 2 : 0) + p * TPV + e / 4][e % 4] : 0.f;
       }
       if (a.partial != nullptr) {                          // rows of whole vectors: ldw is N rounded up to 16
         float* d = a.partial + (((long)split * (a.nout * (DUAL ? 2 : 1)) + which) * a.M + m) * a.ldw + n;
         store_some<float, V>(d, v, a.N - n, aligned && n < a.N);
         if (DUAL) store_some<float, V>(d + a.M * a.ldw, w, a.N - n, aligned && n < a.N);
       } else {
-        epilogue_store<T, DUAL, PLAIN, V>(a.ep, which, m, n, a.N, aligned, v, w, b0, b1);
+        epilogue_store<T, DUAL, PLAIN, V>(a.ep, which, m, n, a.N, aligned, v, w, b0[p], b1[p]);
+      }
+    }
+  };
+  f32x4 sums[NT];
+  if constexpr (CHUNK == 0) {
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) sums[t] = acc[t][u];
+      row(m0 + Q::row_of(qw0, u, i), sums);
+    }
+  } else {
+    f32x4* mine = reinterpret_cast<f32x4*>(lds) + l;
+#pragma unroll
+    for (int u0 = 0; u0 < MT; u0 += CHUNK) {
+#pragma unroll
+      for (int u = 0; u < CHUNK; ++u)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mine[(u * NT + t) * 64] = acc[t][u0 + u];
+#pragma unroll 1
+      for (int u = 0; u < CHUNK; ++u) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sums[t] = mine[(u * NT + t) * 64];
+        row(m0 + Q::row_of(qw0, u0 + u, i), sums);
       }
     }
   }
@@ -341,7 +370,10 @@ __global__ void __launch_bounds__(WN * WM * WK * GROUPS * 64) gemm_kernel(GemmAr
 #pragma unroll
         for (int u = 0; u < MT; ++u) acc[t][u] += join[i * WAVES * 64 * NT * MT + (t * MT + u) * 64];
   }
-  finish<T, P, Q, PKC, QKC, DUAL, NT, MT>(a, acc, n0, pw0, m0, qw0, which, split);
+  constexpr int CHUNK = MT > 1 ? MT : 0;
+  static_assert(CHUNK == 0 || (SETS == 1 && WAVES * NT * CHUNK * 1024 <= RING * GROUPS * SLAB), "sums in LDS");
+  if (CHUNK > 0) __syncthreads();                          // the ring has been read
+  finish<T, P, Q, PKC, QKC, DUAL, NT, MT, CHUNK>(a, acc, n0, pw0, m0, qw0, which, split, lds + wave * NT * CHUNK * 1024);
 }
 
 // ---- large products of 16-bit operands ----------------------------------------------------------------------------------------
@@ -393,7 +425,12 @@ __global__ void __launch_bounds__(WN * WM * 64) gemm_big_kernel(GemmArgs a) {
 
   P pop;
   Q qop;
+  // Each XCD starts at another eighth of k: tiles in step, with rows a power of two apart, ask the same memory channels at the same
+  // time (8192 x 8192 x 8192 forward 872 -> 853 us, 8192 x 4096 x 16384 878 -> 842, bf16; 4096 x 4096 unchanged).
+  const int skew = a.nseg == 1 && tails == 0 && a.splits == 1 ? full * (int)(blockIdx.x % 8) / 8 : 0;
   auto seek = [&](int slab) {
+    slab += skew;
+    if (slab >= all) slab -= all;
     const bool tail = slab < tails;
     const int seg = tail ? slab : full > 0 ? (slab - tails) / full : 0, k0 = (tail ? full : slab - tails - seg * full) * TK;
     pop.init((const T*)a.p[seg], a.ldp[seg], (const T*)a.p[1], a.ldp[1], n0, a.N, k0);
@@ -456,8 +493,13 @@ __global__ void __launch_bounds__(WN * WM * 64) gemm_big_kernel(GemmArgs a) {
       seek(s_begin + RING);
       // slabs until the jump to the second segment (0: none), and its distance from where the first one ends
       int to_jump = a.nseg == 2 ? tails + full - (s_begin + RING) : 0;
-      const long p_jump = a.nseg == 2 ? (const char*)a.p[1] - (const char*)a.p[0] - full * pop.step : 0;
-      const long q_jump = a.nseg == 2 ? (const char*)a.q[1] - (const char*)a.q[0] - full * qop.step : 0;
+      long p_jump = a.nseg == 2 ? (const char*)a.p[1] - (const char*)a.p[0] - full * pop.step : 0;
+      long q_jump = a.nseg == 2 ? (const char*)a.q[1] - (const char*)a.q[0] - full * qop.step : 0;
+      if (skew > 0) {
+        to_jump = full - (s_begin + RING + skew);
+        p_jump = -full * pop.step;
+        q_jump = -full * qop.step;
+      }
       for (int i = 0; i < count - RING; ++i) {
         phase(H0, YES, NO, buf);
         meet<(RING - 2) * LOADS>();                        // the next slab has landed; later ones stay in flight
@@ -477,7 +519,10 @@ __global__ void __launch_bounds__(WN * WM * 64) gemm_big_kernel(GemmArgs a) {
     phase(H0, YES, NO, buf);
     phase(H1, NO, NO, buf);
   }
-  finish<T, P, Q, PKC, QKC, DUAL, NT, MT>(a, acc, n0, pw0, m0, qw0, which, split);
+  constexpr int CHUNK = 4;
+  static_assert(MT % CHUNK == 0 && WN * WM * NT * CHUNK * 1024 <= RING * SLAB, "sums in LDS");
+  __syncthreads();                                         // the ring has been read
+  finish<T, P, Q, PKC, QKC, DUAL, NT, MT, CHUNK>(a, acc, n0, pw0, m0, qw0, which, split, lds + wave * NT * CHUNK * 1024);
 }
 
 template <typename T, int BN, int BM, int WN, int WM, int WK, int GROUPS, int RING> void run_cfg(const GemmArgs& a, hipStream_t s) {

@@ -69,9 +69,19 @@ __global__ void __launch_bounds__(256) join_kernel(GemmArgs a) {
 
 // ---- backward of the activation -----------------------------------------------------------------------------------------
 //   linear:  dz = dy act'(z);      dual:  dg = dy u act'(g), du = dy act(g);      without z: dz = dy
-// z, g and u are the fp32 sums of the forward pass, so dz is rounded once.  The bias gradients are column sums of the
+// z, g and u are the fp32 sums of the forward pass, so dz is rounded once (`two`: and what the rounding took off is kept as well).  The bias gradients are column sums of the
 // unrounded dz: a workgroup adds its rows in registers, then in LDS in a fixed order; `launch_colsum` adds the chunks.
 // Columns N .. ldd-1 of dz are written as zeros (they enter the sums of the products that read dz).
+// what rounding took off v (nothing where it left no finite value: the sum of both parts is that value)
+template <typename T, int V> __device__ __forceinline__ void store_lack(T* dst, const float* v) {
+  float lack[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const float r = to_f(from_f<T>(v[e])), d = v[e] - r;
+    lack[e] = fabsf(r) <= FLT_MAX ? d : 0.f;
+  }
+  store_vec<T, V>(dst, lack);
+}
 template <typename T, bool DUAL>
 __global__ void __launch_bounds__(256) act_bwd_kernel(ActBwdArgs a) {
   constexpr int V = 16 / sizeof(T), TX = 32, TY = 8, D = DUAL ? 2 : 1;
@@ -109,6 +119,10 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(ActBwdArgs a) {
       if (a.dz[0] != nullptr && n < a.ldd) {
         store_vec<T, V>((T*)a.dz[0] + m * a.ldd + n, d0);
         if (DUAL) store_vec<T, V>((T*)a.dz[1] + m * a.ldd + n, d1);
+        if (a.two) {
+          store_lack<T, V>((T*)a.dz[0] + (m + a.M) * a.ldd + n, d0);
+          if (DUAL) store_lack<T, V>((T*)a.dz[1] + (m + a.M) * a.ldd + n, d1);
+        }
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) {
@@ -251,12 +265,13 @@ GemmPlan gemm_plan(int dtype, const GemmArgs& a) {
       const double turns = cfg <= TILE_64x64 ? (per + 1) / 2 * 2 : per;     // slabs in pairs
       double us = 3.5 + turns * f * ((wgs / 2) * c.two + (wgs % 2) * c.one) + wgs * c.end;
       const double floats = (double)splits * a.nout * (a.dual ? 2 : 1) * a.M * best.ldw;
-      if (splits > 1) us += 3.0 + floats * 4 / 2e6;
+      const bool join = splits > 1 || a.halves;
+      if (join) us += 3.0 + floats * 4 / 2e6;
       if (us < best_us) {
         best_us = us;
         best.cfg = cfg;
         best.splits = (int)splits;
-        best.partial_floats = splits > 1 ? (long)floats : 0;
+        best.partial_floats = join ? (long)floats : 0;
       }
     }
   }
@@ -266,12 +281,16 @@ GemmPlan gemm_plan(int dtype, const GemmArgs& a) {
 void launch_gemm(int dtype, GemmArgs a, const GemmPlan& plan, hipStream_t s) {
   a.splits = plan.splits;
   a.ldw = plan.ldw;
-  if (plan.splits == 1) a.partial = nullptr;
+  if (plan.partial_floats == 0) a.partial = nullptr;
   if (dtype == F32) launch_gemm_f32(a, plan.cfg, s);
   else if (dtype == BF16) launch_gemm_bf16(a, plan.cfg, s);
   else launch_gemm_f16(a, plan.cfg, s);
   DDL_HIP_CHECK(hipGetLastError());
-  if (plan.splits > 1) launch_join(dtype, a.partial, a, s);
+  if (a.halves) {                                          // the two halves of the rows lie like two splits
+    a.M /= 2;
+    a.splits *= 2;
+  }
+  if (plan.partial_floats > 0) launch_join(dtype, a.partial, a, s);
 }
 
 }  // namespace ffn

@@ -692,3 +692,41 @@ def test_refusals(dev):
     xg = x.clone().requires_grad_(True)
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(ops.linear(xg, w, activation="gelu").sum(), xg, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("gated", [False, True], ids=["linear", "gated"])
+@pytest.mark.parametrize("M,K,N", [(1, 256, 4), (1, 768, 64), (3, 40, 17), (32, 65, 33)])
+def test_few_rows_round_a_gradient_once(dev, dtype, gated, M, K, N):
+    """Two parts hold dz to u^2 of itself (fp16: to half its smallest step).  Beside that stand dz's own error, from those of z and of
+    the activation, and the fp32 sum over at most 2 x 66 terms; dz's rounding to u is not among them."""
+    from ddl import ops
+    x, w, v = rnd(dev, dtype, M, K), rnd(dev, dtype, N, K, seed=1, scale=K ** -0.5), rnd(dev, dtype, N, K, seed=2, scale=K ** -0.5)
+    dy = rnd(dev, dtype, M, N, seed=3)
+    leaves = [t.requires_grad_(True) for t in ((x, w, v) if gated else (x, w))]
+    y = ops.gated_linear(x, w, v) if gated else ops.linear(x, w, activation="silu")
+    got = torch.autograd.grad(y, leaves, dy)
+    xd, wd, vd, dyd = (t.detach().double() for t in (x, w, v, dy))
+    (z, zerr), (up, uerr) = product_bounds(xd, wd, None, "none"), product_bounds(xd, vd, None, "none")
+    s = torch.sigmoid(z)
+    slope = s * (1 + z * (1 - s))
+    serr, aerr = 1.2 * zerr + 16 * EPS * (1 + z.abs()), 1.13 * zerr + 16 * EPS * z.abs()
+    dz = [dyd * up * slope, dyd * z * s] if gated else [dyd * slope]
+    err = [dyd.abs() * (up.abs() * serr + 1.13 * uerr), dyd.abs() * aerr] if gated else [dyd.abs() * serr]
+    weights = [wd, vd] if gated else [wd]
+    step = tiny(dtype) if dtype == torch.float16 else 0.0
+    err = [e + (oracle.rounding(dtype) ** 2 + 160 * EPS) * d.abs() + step for e, d in zip(err, dz)]
+    close(got[0], sum(d @ p for d, p in zip(dz, weights)), sum(e @ p.abs() for e, p in zip(err, weights)), dtype, "dx")
+    for i, d in enumerate(dz):
+        close(got[1 + i], d.T @ xd, err[i].T @ xd.abs(), dtype, f"dw {i}")
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+def test_few_rows_gradients_that_overflow(dev, dtype):
+    """dz beyond the type's range stays an infinity (what rounding took off it is not another one of the other sign)."""
+    from ddl import ops
+    top = torch.finfo(dtype).max
+    x, w = torch.ones(2, 8, device=dev, dtype=dtype, requires_grad=True), torch.ones(8, 8, device=dev, dtype=dtype, requires_grad=True)
+    y = ops.gated_linear(x, w, w)                          # up 8, gate's slope 1: dg = 8 dy
+    dx, dw = torch.autograd.grad(y, (x, w), torch.full_like(y, top))
+    assert torch.isposinf(dx).all() and torch.isposinf(dw).all()

@@ -8,10 +8,10 @@
 // 4 (t % 2) + i % 4 for tile t, so that a pair of tiles gives eight values; fp32: n = 16 t + i, four values a tile.  Bias, residual
 // and result move as such vectors without a detour through LDS.
 //
-// Tiles: LDS holds a 128-byte wide k slab (64 values of 16 bits, 32 of fp32) of both operands, filled by direct
-// global -> LDS loads of 16 bytes a lane, double buffered: slab t+1 is in flight while slab t is multiplied.  A lane whose
-// 16 bytes lie outside the operand reads a block of zeros in global memory instead, so edges cost no branch and no
-// masked arithmetic, and an infinity beyond the edge cannot turn into NaN.
+// Tiles: LDS holds 128-byte wide k slabs (64 values of 16 bits, 32 of fp32) of both operands in a ring of two or three, filled by
+// direct global -> LDS loads of 16 bytes a lane: the next slabs are in flight while one is multiplied.  A lane whose
+// 16 bytes lie outside the operand reads a block of zeros in global memory instead, so edges cost no masked
+// arithmetic, and an infinity beyond the edge cannot turn into NaN.
 // LDS image of a k-contiguous operand: [row][8 chunks of 16 B]; of a k-strided one: [k][rows].  Chunks are permuted inside a
 // row by an XOR with bits of the row (applied to the global address, since the direct loads write LDS linearly) so that the
 // operand reads spread over the banks.  16-bit k-strided operands are read with the transposing ds_read_b64_tr_b16.
@@ -263,7 +263,10 @@ template <int N> __device__ __forceinline__ void meet() {
 // turn's slabs have landed for everyone, and everyone is done with the previous turn's, whose buffers are filled anew.
 // Small tiles give a CU too little to do: a wave alone on its SIMD stands still in front of every barrier, LDS read and load.  So more
 // waves share a tile along k: WK = 2 groups take one k half of a slab each, and with GROUPS = 2 a turn has two slabs, each staged
-// and multiplied by a group of its own.  Their sums meet in LDS at the end, in a fixed order.
+// and multiplied by a group of its own.  Their sums meet in LDS at the end, in a fixed order.  One slab a turn and one group, bf16:
+// 256 x 4096 x 1024 10.0 us, gated 512 x 1024 x 1024 10.9; two groups 8.3 and 8.6.
+// fp32 is bound by its matrix rate (4096 x 4096 x 4096: 1.06 to 1.12 ms, 123 to 130 TFLOP/s; the library 137), small products by the
+// latency of a load, a barrier and a launch (512 x 1024 x 1024 bf16 7.5 us, fp32 18).
 template <typename T, int BN, int BM, int WN, int WM, int WK, int GROUPS, int RING, bool PKC, bool QKC, bool DUAL>
 __global__ void __launch_bounds__(WN * WM * WK * GROUPS * 64) gemm_kernel(GemmArgs a) {
   constexpr int WAVES = WN * WM, THREADS = WAVES * WK * 64, SETS = WK * GROUPS;
@@ -388,6 +391,9 @@ __global__ void __launch_bounds__(WN * WM * WK * GROUPS * 64) gemm_kernel(GemmAr
 // No edges in the loop: the slab with the end of k comes first (the order of a sum is free), and a tile that would reach beyond the
 // output is moved back inside (it computes some results a second time; both writers hold the same bits).  So N and M are at
 // least a tile.  The second contraction segment has the first one's strides and is reached by a jump.
+// bf16: 8192 x 8192 x 8192 forward 850 us, d_x 795, d_w 825 (1290 to 1380 TFLOP/s; the library 840, 965, 1080); 8192 x 4096 x 4096 205
+// to 215 us in all three directions once the clocks are up (1300; the library 175 to 245).  A CU's fill of LDS, 40 to 47 GB/s, bounds
+// what is left; a ring of 32-value slabs (two barriers for 64 k) reached 783 TFLOP/s where this did 1008.
 template <typename T, int BN, int BM, int WN, int WM, int RING, bool PKC, bool QKC, bool DUAL>
 __global__ void __launch_bounds__(WN * WM * 64) gemm_big_kernel(GemmArgs a) {
   constexpr int THREADS = WN * WM * 64, NT = 4, MT = BM / WM / 16, DBL = 2, SNG = MT - DBL;
@@ -427,7 +433,9 @@ __global__ void __launch_bounds__(WN * WM * 64) gemm_big_kernel(GemmArgs a) {
   Q qop;
   // Each XCD starts at another eighth of k: tiles in step, with rows a power of two apart, ask the same memory channels at the same
   // time (8192 x 8192 x 8192 forward 872 -> 853 us, 8192 x 4096 x 16384 878 -> 842, bf16; 4096 x 4096 unchanged).
-  const int skew = a.nseg == 1 && tails == 0 && a.splits == 1 ? full * (int)(blockIdx.x % 8) / 8 : 0;
+  // Only where no tile was moved: both writers of an output have to sum in the same order.
+  const bool whole = a.N % TN == 0 && a.M % BM == 0 && tails == 0;
+  const int skew = whole && a.nseg == 1 && a.splits == 1 ? full * (int)(blockIdx.x % 8) / 8 : 0;
   auto seek = [&](int slab) {
     slab += skew;
     if (slab >= all) slab -= all;

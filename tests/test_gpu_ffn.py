@@ -730,3 +730,41 @@ def test_few_rows_gradients_that_overflow(dev, dtype):
     y = ops.gated_linear(x, w, w)                          # up 8, gate's slope 1: dg = 8 dy
     dx, dw = torch.autograd.grad(y, (x, w), torch.full_like(y, top))
     assert torch.isposinf(dx).all() and torch.isposinf(dw).all()
+
+
+@pytest.mark.parametrize("M,K,N", [(2500, 4096, 2500), (2100, 2048, 4200), (2560, 4096, 2816)])
+def test_large_products_repeat_bit_for_bit(dev, M, K, N):
+    """Tiles that reach beyond the output are moved inside it: some results have two writers."""
+    from ddl import ops
+    x, w = (rnd(dev, torch.bfloat16, *s, seed=1).requires_grad_(True) for s in ((M, K), (N, K)))
+    dy = rnd(dev, torch.bfloat16, M, N, seed=2)
+
+    def step():
+        y = ops.linear(x, w, activation="relu")
+        return (y.detach(),) + torch.autograd.grad(y, (x, w), dy)
+
+    want = step()
+    for _ in range(6):
+        assert all(torch.equal(a, b) for a, b in zip(step(), want))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("M", [3, 130])
+def test_one_tensor_in_several_places_and_a_graph_walked_twice(dev, dtype, M):
+    from ddl import ops
+    C = 40
+    x, w = rnd(dev, dtype, M, C).requires_grad_(True), rnd(dev, dtype, C, C, seed=1, scale=C ** -0.5).requires_grad_(True)
+    parts = [x.detach().clone().requires_grad_(True), x.detach().clone().requires_grad_(True)]
+    weights = [w.detach().clone().requires_grad_(True) for _ in range(3)]
+    y = ops.linear(ops.gated_linear(x, w, w), w, residual=x)
+    z = ops.linear(ops.gated_linear(parts[0], weights[0], weights[1]), weights[2], residual=parts[1])
+    assert torch.equal(y, z)
+    dy = torch.ones((), device=dev, dtype=dtype).expand(M, C)
+    first = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    again = torch.autograd.grad(y, (x, w), dy)
+    assert all(torch.equal(s, t) for s, t in zip(first, again))
+    each = torch.autograd.grad(z, parts + weights, dy)
+    u = oracle.rounding(dtype)
+    for got, terms in zip(first, (each[:2], each[2:])):              # a sum of two or three rounds twice at most, in any order
+        total, mag = sum(t.double() for t in terms), sum(t.double().abs() for t in terms)
+        assert ((got.double() - total).abs() <= 2.1 * u * mag + tiny(dtype)).all()

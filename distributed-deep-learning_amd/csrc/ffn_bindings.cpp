@@ -70,17 +70,6 @@ bool is_operand(const Tensor& t) {
   const int64_t epc = 16 / t.element_size();
   return t.numel() == 0 || ((t.size(1) <= 1 || t.stride(1) == 1) && t.size(1) % epc == 0 && rows_aligned(t));
 }
-// t's rows into rows `row` .. of a buffer with rows of ld elements
-void pack_rows(const Tensor& t, void* dst, long row, long ld, ffn::PackArgs& todo) {
-  ffn::PackItem& it = todo.item[todo.count++];
-  it.src = t.data_ptr();
-  it.dst = (char*)dst + row * ld * t.element_size();
-  it.s_row = t.stride(0);
-  it.s_col = t.stride(1);
-  it.ld = ld;
-  it.rows = t.size(0);
-  it.cols = (int)t.size(1);
-}
 // t: 2-D [rows, width], or packed already.  What has to be packed joins `todo`, for one launch.
 Operand operand(const Tensor& t, int64_t width, ffn::PackArgs& todo) {
   Operand o;
@@ -98,8 +87,15 @@ Operand operand(const Tensor& t, int64_t width, ffn::PackArgs& todo) {
   }
   o.ld = line(t.size(1), t);
   o.keep = at::empty({t.size(0), o.ld}, t.options());
+  ffn::PackItem& it = todo.item[todo.count++];
+  it.src = t.data_ptr();
+  it.dst = o.keep.data_ptr();
+  it.s_row = t.stride(0);
+  it.s_col = t.stride(1);
+  it.ld = o.ld;
+  it.rows = t.size(0);
+  it.cols = (int)t.size(1);
   o.p = o.keep.data_ptr();
-  pack_rows(t, o.keep.data_ptr(), 0, o.ld, todo);
   return o;
 }
 Operand own_operand(const Tensor& padded) {                          // a padded buffer of ours
@@ -247,9 +243,9 @@ ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width,
   // rounding that makes a gradient's error sqrt(2) times one rounding, where many of them average.  Few rows may not average (one
   // row, 64 columns: 1.57 times the rounding alone, four columns: 3), and their products have time to spare.  So up to FEW_ROWS rows
   // dz comes in two parts, the rounded one in rows 0 .. M-1 and what it lacks in rows M .. 2M-1: d_x sums both rows' outputs in
-  // fp32 before it rounds, d_w contracts over all of them with x twice.
+  // fp32 before it rounds, d_w adds the parts before it multiplies.
   const bool make_dz = z.defined() && (need_dx || need_dw);
-  const bool two = make_dz && dtype != ffn::F32 && M <= ffn::FEW_ROWS;
+  const bool few = M <= ffn::FEW_ROWS, two = make_dz && dtype != ffn::F32 && few;
   const int R = two ? 2 * M : M;
   Tensor dz;
   Operand dzo[2], wo[2], xo;
@@ -257,19 +253,14 @@ ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width,
   if (make_dz) {
     dz = at::empty({D, R, line(N, x)}, x.options());
     for (int d = 0; d < D; ++d) dzo[d] = own_operand(dz[d]);
-  } else if (need_dx || need_dw) {
+  } else if (need_dx || (need_dw && !few)) {
     dzo[0] = operand(dy2, N, todo);
   }
   if (K > 0 && need_dx) {
     wo[0] = operand(rows_of(w0), K, todo);
     if (dual) wo[1] = operand(rows_of(w1), K, todo);
   }
-  if (K > 0 && need_dw && two) {
-    xo = own_operand(at::empty({R, line(K, x)}, x.options()));
-    for (long half = 0; half < 2; ++half) pack_rows(x2, const_cast<void*>(xo.p), half * M, xo.ld, todo);
-  } else if (K > 0 && need_dw) {
-    xo = operand(x2, K, todo);
-  }
+  if (K > 0 && need_dw && !few) xo = operand(x2, K, todo);
   ffn::launch_pack(dtype, todo, cur_stream());
   if (make_dz || need_db) {
     ffn::ActBwdArgs b;
@@ -316,9 +307,24 @@ ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width,
     set_out(g.ep, 0, r.dx);
     run_gemm(dtype, g, x);
   }
-  if (need_dw) {                                                     // dw[n][k] = sum over m of dz[m][n] x[m][k]
+  if (need_dw && few) {
+    ffn::OuterArgs o;
+    o.M = M; o.N = N; o.K = K;
+    o.nout = D;
+    o.x = x2.data_ptr();
+    o.ldx = row_stride(x2);
+    o.x_vec = rows_aligned(x2);
+    o.two = two;
+    o.ldd = make_dz ? dzo[0].ld : row_stride(dy2);
+    o.out_vec = (int64_t)K * x.element_size() % 16 == 0;
+    for (int d = 0; d < D; ++d) {
+      o.dz[d] = make_dz ? dzo[d].p : dy2.data_ptr();
+      o.out[d] = r.dw[d].data_ptr();
+    }
+    ffn::launch_outer(dtype, o, cur_stream());
+  } else if (need_dw) {                                              // dw[n][k] = sum over m of dz[m][n] x[m][k]
     ffn::GemmArgs g;
-    g.N = K; g.M = N; g.K = R;
+    g.N = K; g.M = N; g.K = M;
     g.nout = D;
     g.p_kc = g.q_kc = false;
     g.p[0] = xo.p; g.ldp[0] = xo.ld;

@@ -223,6 +223,17 @@ struct ActBwdArgs {
   void* db[2] = {nullptr, nullptr};       // instead, with one chunk: the column sums themselves, in the element type
   int chunks = 0;
 };
+// few rows: out[which][n][k] = sum over m of dz[which][m][n] x[m][k], rows of K; two: dz in two parts (see above)
+struct OuterArgs {
+  const void* dz[2] = {nullptr, nullptr};
+  const void* x = nullptr;
+  void* out[2] = {nullptr, nullptr};
+  long ldd = 0, ldx = 0;
+  int M = 0, N = 0, K = 0, nout = 1;
+  int rows = 0, strips = 0;               // of the output: rows a workgroup writes, strips of 1024 columns (the launcher's)
+  bool two = false, x_vec = false, out_vec = false;
+};
+void launch_outer(int dtype, const OuterArgs& a, hipStream_t s);
 int act_bwd_chunks(int dtype, int M, int N);
 void launch_act_bwd(int dtype, const ActBwdArgs& a, hipStream_t s);
 // out[which][n] = sum over chunks of part[chunk][which][n]

@@ -768,3 +768,13 @@ def test_one_tensor_in_several_places_and_a_graph_walked_twice(dev, dtype, M):
     for got, terms in zip(first, (each[:2], each[2:])):              # a sum of two or three rounds twice at most, in any order
         total, mag = sum(t.double() for t in terms), sum(t.double().abs() for t in terms)
         assert ((got.double() - total).abs() <= 2.1 * u * mag + tiny(dtype)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("M", [2, 4, 7, 8, 9, 12, 13, 16, 17, 24, 25, 31, 33])
+def test_every_count_of_few_rows(dev, dtype, M):
+    """Row counts on both sides of each variant's limit, a width beyond one strip of columns and off every vector."""
+    K, N = 2051, 77
+    x, w, b = rnd(dev, dtype, M, K, seed=1), rnd(dev, dtype, N, K, seed=2, scale=K ** -0.5), rnd(dev, dtype, N, seed=3)
+    for act in ("none", "silu"):
+        check_linear(dev, dtype, x, w, b, act, None)

@@ -1,4 +1,4 @@
-// Products with few rows (inference on one or a few rows): out[m][n] = epilogue(sum_k w(n, k) x(m, k)), m < 32.
+// Products with few rows (inference on one or a few rows): out[m][n] = epilogue(sum_k w(n, k) x(m, k)), up to 32 rows m.
 //
 // Bound by reading the weights once: 2 N K bytes in 16 bits against 2 M N K operations.  A workgroup owns 16 weight rows and
 // streams them from memory straight into the matrix cores' A operand (lane: 16 bytes of one row), eight waves splitting k;
@@ -99,10 +99,13 @@ template <typename T> void run(const FewRowsArgs& a, hipStream_t s) {
     if (a.M <= 16) run_vec<T, 1, false>(a, s); else run_vec<T, 2, false>(a, s);
   }
 }
+
 // ---- the weights' gradient of few rows: a sum of outer products --------------------------------------------------------------
-// Bound by writing the result: 2 M operations an output.  A thread keeps four or eight columns of x in registers, all rows of them, and walks
-// down the rows of the result; dz lies in LDS as [row of the result][m] and is read by all lanes at once; a wave writes 64 such runs.  Tiles on the matrix cores live for one slab here and wait for it: gated 10 x 9408 x 6080 fp32 234 us there
-// and 97 here (457 MB, 4.7 TB/s), 30 x 4096 x 4096 73 and 49, bf16 1 x 11264 x 4096 57 and 51, 10 x 9408 x 6080 72 and 75 (act' included).
+// Bound by writing the result: 2 M operations an output.  A thread keeps four or eight columns of x in registers, all rows of them, and
+// walks down the rows of the result; dz lies in LDS as [row of the result][m] and is read by all lanes at once; a wave writes 64
+// such runs.  A tile on the matrix cores would live for one slab and wait for it.  Tiles and this, the activation's gradient
+// included: gated 10 x 9408 x 6080 fp32 234 us and 97 (457 MB, 4.7 TB/s), 30 x 4096 x 4096 73 and 49; bf16 1 x 11264 x 4096 57 and
+// 51, 10 x 9408 x 6080 72 and 75.
 // `two`: both parts of dz are added in fp32 first.
 template <typename T, int V, int MR>
 __global__ void __launch_bounds__(256) outer_kernel(OuterArgs a) {

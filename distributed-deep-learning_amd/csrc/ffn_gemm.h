@@ -264,7 +264,8 @@ template <int N> __device__ __forceinline__ void meet() {
 // Small tiles give a CU too little to do: a wave alone on its SIMD stands still in front of every barrier, LDS read and load.  So more
 // waves share a tile along k: WK = 2 groups take one k half of a slab each, and with GROUPS = 2 a turn has two slabs, each staged
 // and multiplied by a group of its own.  Their sums meet in LDS at the end, in a fixed order.  One slab a turn and one group, bf16:
-// 256 x 4096 x 1024 10.0 us, gated 512 x 1024 x 1024 10.9; two groups 8.3 and 8.6.
+// 256 x 4096 x 1024 10.0 us, gated 512 x 1024 x 1024 10.9; two groups 8.3 and 8.6.  A ring of three turns for 64 x 64 leaves a CU one
+// workgroup instead of two: 512 x 4096 x 1024 bf16 13.6 us with two, 20.8 with three.
 // fp32 is bound by its matrix rate (4096 x 4096 x 4096: 1.06 to 1.12 ms, 123 to 130 TFLOP/s; the library 137), small products by the
 // latency of a load, a barrier and a launch (512 x 1024 x 1024 bf16 7.5 us, fp32 18).
 template <typename T, int BN, int BM, int WN, int WM, int WK, int GROUPS, int RING, bool PKC, bool QKC, bool DUAL>

@@ -203,6 +203,7 @@ __device__ __forceinline__ void finish(const GemmArgs& a, const f32x4 (&acc)[NT]
       if (DUAL) load_bias<T, V>(a.ep, 1, n1 + 4 * V * p, a.N, aligned, b1[p]);
     }
   }
+  constexpr bool Z_ROWS = DUAL && CHUNK > 0;               // z is written by itself below
   // the sums of row m
   auto row = [&](int m, const f32x4 (&sums)[NT]) {
     if (m >= a.M) return;
@@ -220,7 +221,13 @@ __device__ __forceinline__ void finish(const GemmArgs& a, const f32x4 (&acc)[NT]
         store_some<float, V>(d, v, a.N - n, aligned && n < a.N);
         if (DUAL) store_some<float, V>(d + a.M * a.ldw, w, a.N - n, aligned && n < a.N);
       } else {
-        epilogue_store<T, DUAL, PLAIN, V>(a.ep, which, m, n, a.N, aligned, v, w, b0[p], b1[p]);
+        if constexpr (Z_ROWS) {
+          Epilogue ep = a.ep;
+          ep.z[0] = nullptr;
+          epilogue_store<T, DUAL, PLAIN, V>(ep, which, m, n, a.N, aligned, v, w, b0[p], b1[p]);
+        } else {
+          epilogue_store<T, DUAL, PLAIN, V>(a.ep, which, m, n, a.N, aligned, v, w, b0[p], b1[p]);
+        }
       }
     }
   };
@@ -233,6 +240,15 @@ __device__ __forceinline__ void finish(const GemmArgs& a, const f32x4 (&acc)[NT]
       row(m0 + Q::row_of(qw0, u, i), sums);
     }
   } else {
+    // z of dual products: 16 lanes take the 2 x 32 sums of a row, four each (16 bits: tile t holds columns 32 (t / 2) + 8 kg + 4 (t % 2);
+    // fp32: 16 t + 4 kg), so that a store covers whole lines; as the lanes hold them, 16 of every 32 bytes.  Keeping the sums
+    // adds 30 us to 2011 x 2708 x 1000 bf16 the latter way, 16 by rows.  Single products keep the lanes' way: a training step over
+    // 8192 x 4096 x 4096 took 754 us with it, 806 by rows.
+    const int zq = l & 15, zt = V == 8 ? 2 * (zq >> 3) + (zq & 1) : zq >> 2, zkg = V == 8 ? (zq & 7) >> 1 : zq & 3;
+    const bool up = zt >= NT / 2, keep = Z_ROWS && a.ep.z[0] != nullptr && a.partial == nullptr;
+    const int zn = n0 + pw0 + 4 * (zq & 7);
+    float zb[4] = {0.f, 0.f, 0.f, 0.f};
+    if (keep) load_bias<T, 4>(a.ep, up, zn, a.N, aligned, zb);
     f32x4* mine = reinterpret_cast<f32x4*>(lds) + l;
 #pragma unroll
     for (int u0 = 0; u0 < MT; u0 += CHUNK) {
@@ -242,6 +258,17 @@ __device__ __forceinline__ void finish(const GemmArgs& a, const f32x4 (&acc)[NT]
         for (int t = 0; t < NT; ++t) mine[(u * NT + t) * 64] = acc[t][u0 + u];
 #pragma unroll 1
       for (int u = 0; u < CHUNK; ++u) {
+        if (keep) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int zi = 4 * j + (l >> 4), m = m0 + Q::row_of(qw0, u0 + u, zi);
+            const f32x4 q = reinterpret_cast<f32x4*>(lds)[(u * NT + zt) * 64 + zkg * 16 + zi];
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = q[e] + zb[e];
+            if (m < a.M && zn < a.N) store_some<float, 4>(a.ep.z[up] + m * a.ep.ldz + zn, v, a.N - zn, aligned);
+          }
+        }
 #pragma unroll
         for (int t = 0; t < NT; ++t) sums[t] = mine[(u * NT + t) * 64];
         row(m0 + Q::row_of(qw0, u0 + u, i), sums);

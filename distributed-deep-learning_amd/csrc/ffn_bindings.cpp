@@ -60,8 +60,10 @@ bool rows_aligned(const Tensor& t) {
 // An operand of a product: 16-byte aligned rows of whole 16-byte chunks.  A tensor that is not laid out so (odd widths, a column
 // slice, a transposed view) is packed into a copy whose rows are padded with zeros to 128 bytes, one pass over it.  Training
 // keeps the copy instead of the tensor, so the backward pass finds it packed: [rows, padded] with the width known from elsewhere.
+// An operand owns the tensor it is packed from: the packing launch comes after all operands are set up, and memory given back before
+// it could become one of the others' copies.
 struct Operand {
-  Tensor keep;
+  Tensor keep, source;
   const void* p = nullptr;
   long ld = 0;
 };
@@ -70,9 +72,10 @@ bool is_operand(const Tensor& t) {
   const int64_t epc = 16 / t.element_size();
   return t.numel() == 0 || ((t.size(1) <= 1 || t.stride(1) == 1) && t.size(1) % epc == 0 && rows_aligned(t));
 }
-// t: 2-D [rows, width], or packed already.  What has to be packed joins `todo`, for one launch.
+// t: 2-D [rows, width] of any strides, or packed already.  What has to be packed joins `todo`, for one launch.
 Operand operand(const Tensor& t, int64_t width, ffn::PackArgs& todo) {
   Operand o;
+  o.source = t;
   if (t.size(1) != width) {
     o.keep = t;
     o.p = t.data_ptr();
@@ -257,8 +260,8 @@ ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width,
     dzo[0] = operand(dy2, N, todo);
   }
   if (K > 0 && need_dx) {
-    wo[0] = operand(rows_of(w0), K, todo);
-    if (dual) wo[1] = operand(rows_of(w1), K, todo);
+    wo[0] = operand(w0, K, todo);
+    if (dual) wo[1] = operand(w1, K, todo);
   }
   if (K > 0 && need_dw && !few) xo = operand(x2, K, todo);
   ffn::launch_pack(dtype, todo, cur_stream());

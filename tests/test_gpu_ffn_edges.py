@@ -1,0 +1,67 @@
+"""Calls of the feed-forward operators that their documentation allows and tests/test_gpu_ffn.py does not make: more than one operand
+in an unusual layout, the explicit forward / backward pairs, sizes at the limits.  Bounds are those of tests/test_gpu_ffn.py.
+"""
+import pytest
+import torch
+
+import ffn_oracle as oracle
+from test_gpu_ffn import EPS, IDS, TYPES, check_gated, check_linear, close, rnd
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "gpu tests need a GPU"
+    from ddl import ops
+    ops.require_ext()
+    return torch.device("cuda", 0)
+
+
+@pytest.fixture(scope="module")
+def ext(dev):
+    from ddl import ops
+    return ops.require_ext()
+
+
+# ---- operands that need both a change of layout and padding ------------------------------------------------------------------
+def strided(t, how):
+    """t's values behind strides that a product cannot read in place"""
+    if how == "transposed":
+        return t.t().contiguous().t()
+    wide = torch.empty(t.shape[0], 2 * t.shape[1], dtype=t.dtype, device=t.device)
+    v = wide[:, ::2]
+    v.copy_(t)
+    return v
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("how", ["transposed", "every other column"])
+@pytest.mark.parametrize("M", [1, 5, 32, 33, 90])
+@pytest.mark.parametrize("K", [41, 56])
+def test_all_operands_strided_at_once(dev, dtype, how, M, K):
+    N = 40
+    x, g, u = (rnd(dev, dtype, *s, seed=i, scale=c) for i, (s, c) in enumerate((((M, K), 1.0), ((N, K), 0.2), ((N, K), 0.2))))
+    check_gated(dev, dtype, *(strided(t, how) for t in (x, g, u)), None, None, "gelu")
+    check_linear(dev, dtype, strided(x, how), strided(g, how), None, "silu", strided(rnd(dev, dtype, M, N, seed=4), how))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("M", [3, 32, 40, 200])
+def test_explicit_pairs_with_strided_operands(dev, ext, dtype, M):
+    """The pairs that the model's units call: strided tensors give the bits that contiguous ones give."""
+    K, N = 41, 27
+    x, g, u, dy = (rnd(dev, dtype, *s, seed=i) for i, s in enumerate(((M, K), (N, K), (N, K), (M, N))))
+    silu = 2
+
+    def both(x, g, u, dy):
+        h, z = ext.gated_forward(x, g, u, None, None, silu, True)
+        y, s = ext.linear_forward(x, g, None, None, silu, True)
+        out = [h, y] + list(ext.gated_backward(dy, x, g, u, z, silu, True, True, True))
+        out += list(ext.linear_backward(dy, x, g, s, silu, True, True, True))
+        return out + list(ext.linear_backward(dy, x, g, None, 0, True, True, True))
+
+    want = both(x, g, u, dy)
+    for how in ("transposed", "every other column"):
+        for got, w in zip(both(*(strided(t, how) for t in (x, g, u, dy))), want):
+            assert torch.equal(got, w), how

@@ -371,6 +371,14 @@ void check_dy(const Tensor& dy, const Tensor& x, int64_t n, const char* op) {
   check_like(dy, x, op, "the output's gradient");
   BAD_UNLESS(dy.sizes().vec() == out_sizes(x, n), op, ": gradient ", dy.sizes(), " where the result is ", out_sizes(x, n));
 }
+// the sums that the forward pass keeps: fp32 [planes, rows of x, n rounded up to 16]
+void check_kept(const Tensor& z, int64_t planes, const Tensor& x, int64_t n, const char* op) {
+  int64_t rows = 1;                                                  // not numel / K: K may be zero
+  for (int64_t d = 0; d + 1 < x.dim(); ++d) rows *= x.size(d);
+  BAD_UNLESS(z.defined() && z.is_contiguous() && z.scalar_type() == at::kFloat && z.dim() == 3 && z.size(0) == planes &&
+                 z.size(1) == rows && z.size(2) == up(n, 16) && z.device() == x.device(),
+             op, ": the backward pass needs the sums kept by the forward pass of the same call");
+}
 std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& dy, const Tensor& x, const Tensor& w, const OptT& z, int64_t act,
                                                    bool need_dx, bool need_dw, bool need_db) {
   check_linear(x, w, OptT(), OptT(), act);
@@ -378,10 +386,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& dy, const Tenso
   BAD_UNLESS(act == ffn::ACT_NONE || has(z), "linear: the backward pass of an activation needs the sums kept by the forward pass");
   ddl::DeviceGuard guard(x.device());
   const Tensor zz = act == ffn::ACT_NONE ? Tensor() : get(z);
-  if (zz.defined())
-    BAD_UNLESS(zz.is_contiguous() && zz.scalar_type() == at::kFloat && zz.dim() == 3 && zz.size(0) == 1 &&
-                   zz.size(1) * x.size(-1) == x.numel() && zz.size(2) == up(w.size(0), 16) &&
-                   zz.device() == x.device(), "linear: kept sums of another call");
+  if (zz.defined()) check_kept(zz, 1, x, w.size(0), "linear");
   auto r = product_backward(dy, {zz, x, {w, Tensor()}}, x.size(-1), (int)act, need_dx, need_dw, need_db, "linear");
   return {need_dx ? r.dx.view(x.sizes()) : r.dx, r.dw[0], r.db[0]};
 }
@@ -457,9 +462,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_backward(const Tensor& 
                                                                   bool need_dw, bool need_db) {
   check_gated(x, wg, wu, OptT(), OptT(), act);
   check_dy(dy, x, wg.size(0), "gated_linear");
-  BAD_UNLESS(z.defined() && z.is_contiguous() && z.scalar_type() == at::kFloat && z.dim() == 3 && z.size(0) == 2 &&
-                 z.size(1) * x.size(-1) == x.numel() && z.size(2) == up(wg.size(0), 16) && z.device() == x.device(),
-             "gated_linear: the backward pass needs the sums kept by the forward pass");
+  check_kept(z, 2, x, wg.size(0), "gated_linear");
   ddl::DeviceGuard guard(x.device());
   auto r = product_backward(dy, {z, x, {wg, wu}}, x.size(-1), (int)act, need_dx, need_dw, need_db, "gated_linear");
   return {need_dx ? r.dx.view(x.sizes()) : r.dx, r.dw[0], r.dw[1], r.db[0], r.db[1]};

@@ -65,3 +65,18 @@ def test_explicit_pairs_with_strided_operands(dev, ext, dtype, M):
     for how in ("transposed", "every other column"):
         for got, w in zip(both(*(strided(t, how) for t in (x, g, u, dy))), want):
             assert torch.equal(got, w), how
+
+
+def test_kept_sums_of_another_call_are_refused(dev, ext):
+    """Also where nothing is summed (K = 0), so that the number of rows cannot be told from the number of elements."""
+    for K in (0, 8):
+        few, many, w = (torch.zeros(n, K, device=dev) for n in (3, 50, 7))
+        dy = torch.zeros(50, 7, device=dev)
+        _, z = ext.linear_forward(few, w, None, None, 2, True)
+        _, zz = ext.gated_forward(few, w, w, None, None, 2, True)
+        with pytest.raises(ValueError, match="kept"):
+            ext.linear_backward(dy, many, w, z, 2, True, True, True)
+        with pytest.raises(ValueError, match="kept"):
+            ext.gated_backward(dy, many, w, w, zz, 2, True, True, True)
+        with pytest.raises(ValueError, match="kept"):
+            ext.gated_backward(dy[:3], few, w, w, z, 2, True, True, True)

@@ -35,6 +35,16 @@ const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 long up(long n, long to) { return (n + to - 1) / to * to; }
 
+// The operators have a backward pass and no forward-mode derivative.  Their kernels see values only, so a tangent would be lost without a
+// word: a call on a dual tensor is refused.
+void no_tangent(const Tensor& t, const char* op) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), op,
+                              ": no forward-mode derivative (an argument is a dual tensor of torch.autograd.forward_ad)");
+}
+void no_tangents(std::initializer_list<const Tensor*> ts, const char* op) {
+  for (const Tensor* t : ts) no_tangent(*t, op);
+}
+
 // `t` may stand beside `x` in a call: same device and type
 void check_like(const Tensor& t, const Tensor& x, const char* op, const char* name) {
   BAD_UNLESS(t.device() == x.device(), op, ": ", name, " is on ", t.device(), ", the input on ", x.device());
@@ -352,6 +362,8 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
 
 // what linear checks; then the pieces that the model's units call: forward -> (y, z), backward -> (dx, dw, db)
 void check_linear(const Tensor& x, const Tensor& w, const OptT& b, const OptT& res, int64_t act) {
+  const Tensor bias = get(b), residual = get(res);
+  no_tangents({&x, &w, &bias, &residual}, "linear");
   check_product(x, w, b, "linear", "weight", "bias");
   check_act(act, "linear");
   if (has(res)) {
@@ -368,6 +380,7 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, cons
   return {y.view(out_sizes(x, w.size(0))), kept.z};
 }
 void check_dy(const Tensor& dy, const Tensor& x, int64_t n, const char* op) {
+  no_tangent(dy, op);
   check_like(dy, x, op, "the output's gradient");
   BAD_UNLESS(dy.sizes().vec() == out_sizes(x, n), op, ": gradient ", dy.sizes(), " where the result is ", out_sizes(x, n));
 }
@@ -424,6 +437,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_second_derivative("linear");
     if (!grads[0].defined()) return variable_list(5);
+    no_tangent(grads[0], "linear");
     const auto saved = ctx->get_saved_variables();
     const Needs need(ctx);
     ddl::DeviceGuard guard(grads[0].device());
@@ -443,6 +457,8 @@ Tensor linear(const Tensor& x, const Tensor& w, const OptT& b, const OptT& res, 
 }
 
 void check_gated(const Tensor& x, const Tensor& wg, const Tensor& wu, const OptT& bg, const OptT& bu, int64_t act) {
+  const Tensor b0 = get(bg), b1 = get(bu);
+  no_tangents({&x, &wg, &wu, &b0, &b1}, "gated_linear");
   check_product(x, wg, bg, "gated_linear", "w_gate", "b_gate");
   check_product(x, wu, bu, "gated_linear", "w_up", "b_up");
   BAD_UNLESS(wg.sizes() == wu.sizes(), "gated_linear: w_gate ", wg.sizes(), " and w_up ", wu.sizes(), " differ");
@@ -484,6 +500,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_second_derivative("gated_linear");
     if (!grads[0].defined()) return variable_list(6);
+    no_tangent(grads[0], "gated_linear");
     const auto s = ctx->get_saved_variables();
     const Needs need(ctx);
     ddl::DeviceGuard guard(grads[0].device());
@@ -506,6 +523,8 @@ Tensor gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu, const O
 
 // ---- dropout ------------------------------------------------------------------------------------------------------------
 void check_dropout(const Tensor& x, double p, const Tensor& key, const OptT& res) {
+  no_tangent(x, "dropout");
+  no_tangent(get(res), "dropout");
   BAD_UNLESS(x.is_cuda(), "dropout: GPU tensor expected");
   type_of(x, "dropout");
   BAD_UNLESS(p >= 0. && p <= 1., "dropout: p must lie in [0, 1], got ", p);
@@ -543,6 +562,7 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_second_derivative("dropout");
     if (!grads[0].defined()) return variable_list(4);
+    no_tangent(grads[0], "dropout");
     const Needs need(ctx);
     Tensor dx;
     if (need(0))
@@ -577,6 +597,7 @@ struct NormIn {
 struct NormSetup { ffn::NormArgs a; Tensor keep[8]; int dtype = 0; };
 NormSetup norm_setup(const NormIn& in) {
   const char* op = "residual_norm";
+  no_tangents({&in.x, &in.y, &in.gate, &in.post_w, &in.post_b, &in.pre_w, &in.pre_b}, op);
   BAD_UNLESS(in.x.is_cuda(), op, ": GPU tensor expected");
   NormSetup s;
   s.dtype = type_of(in.x, op);
@@ -672,6 +693,7 @@ NormGrads norm_backward(const NormIn& in, const Tensor& st, const Tensor& dr, co
   Tensor drc, dhc;
   auto grad = [&](const Tensor& t, Tensor& c) -> const void* {
     if (!t.defined()) return nullptr;
+    no_tangent(t, "residual_norm");
     check_like(t, in.x, "residual_norm", "an output's gradient");
     BAD_UNLESS(t.sizes() == in.x.sizes(), "residual_norm: gradient ", t.sizes(), " where x is ", in.x.sizes());
     c = t.contiguous();

@@ -7,7 +7,7 @@ Together they are the residual block of a model's trunk or head::
     y = dropout(y, p, rng.next_key())                              # the mask is regenerated, never stored
     x, n = residual_norm(x, y, pre_weight=w, gate=g)               # join, and the next block's norm, in one pass
 
-All four are differentiable once, take float32, bfloat16 and float16 (one type per call; the vectors of ``residual_norm`` may be
+All four are differentiable once, by a backward pass (forward-mode tangents are refused on the GPU), take float32, bfloat16 and float16 (one type per call; the vectors of ``residual_norm`` may be
 float32 beside 16-bit rows) and inputs of any strides, sum in fp32, and round a result once.  On the GPU they run the kernels of
 ``csrc/ffn_*.hip`` on the current stream and can be captured into a graph; on the CPU the same functions are plain PyTorch.
 Arguments that do not fit raise ``ValueError``.

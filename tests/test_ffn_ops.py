@@ -97,3 +97,37 @@ def test_refusals():
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+def test_forward_mode_is_right_or_refused():
+    """The plain path has tangents; the kernels have none and refuse a dual tensor, before they look at anything else of it."""
+    import torch.autograd.forward_ad as fwd
+    x, w, b = rnd(torch.float32, 4, 8, seed=1), rnd(torch.float32, 8, 8, seed=2), rnd(torch.float32, 8, seed=3)
+    v, key = torch.ones(8), torch.tensor([1, 2])
+    with fwd.dual_level():
+        for i in range(3):
+            a = [x, w, b]
+            t = torch.ones_like(a[i])
+            a[i] = fwd.make_dual(a[i], t)
+            got = fwd.unpack_dual(ops.linear(*a)).tangent
+            want = (lambda: t @ w.T, lambda: x @ t.T, lambda: t.expand(4, 8))[i]()
+            same(got, want.double(), torch.float32, 64.0)
+        ext = ops.load_ext()
+        if ext is None:
+            pytest.skip("extension not built")
+        d, dw, db = (fwd.make_dual(t, torch.ones_like(t)) for t in (x, w, b))
+        dv = fwd.make_dual(v, v)
+        norm = [x, x, v, v, v, v, v]
+        calls = [lambda: ext.linear(d, w, b, x, 0), lambda: ext.linear(x, dw, b, x, 0), lambda: ext.linear(x, w, db, x, 0),
+                 lambda: ext.linear(x, w, b, d, 0), lambda: ext.linear_forward(d, w, b, x, 0, False),
+                 lambda: ext.gated_linear(d, w, w, b, b, 2), lambda: ext.gated_linear(x, dw, w, b, b, 2),
+                 lambda: ext.gated_linear(x, w, dw, b, b, 2), lambda: ext.gated_linear(x, w, w, db, b, 2),
+                 lambda: ext.gated_linear(x, w, w, b, db, 2), lambda: ext.dropout(d, 0.5, key, None), lambda: ext.dropout(x, 0.5, key, d)]
+        for i in range(7):
+            args = list(norm)
+            args[i] = d if i < 2 else dv
+            calls.append(lambda args=args: ext.residual_norm(*args, True, 1e-6, 1.0))
+        for i, call in enumerate(calls):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+                pytest.fail(f"call {i} was not refused")

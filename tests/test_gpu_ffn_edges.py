@@ -80,3 +80,23 @@ def test_kept_sums_of_another_call_are_refused(dev, ext):
             ext.gated_backward(dy, many, w, w, zz, 2, True, True, True)
         with pytest.raises(ValueError, match="kept"):
             ext.gated_backward(dy[:3], few, w, w, z, 2, True, True, True)
+
+
+def test_dual_tensors_are_refused(dev):
+    """No leaf requires a gradient, so no autograd node stands in the way: the result would have no tangent."""
+    import torch.autograd.forward_ad as fwd
+    from ddl import ops
+    x, w = rnd(dev, torch.float32, 40, 8), rnd(dev, torch.float32, 8, 8, seed=1)
+    key, v = torch.tensor([1, 2], device=dev), torch.ones(8, device=dev)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops.linear(d, w), lambda: ops.linear(x, w, residual=d), lambda: ops.gated_linear(d, w, w),
+                     lambda: ops.dropout(d, 0.5, key), lambda: ops.residual_norm(d, pre_weight=v), lambda: ops.residual_norm(x, d)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        # a dual gradient of an ordinary result
+        leaf = x.clone().requires_grad_(True)
+        for y in (ops.linear(leaf, w, activation="silu"), ops.gated_linear(leaf, w, w), ops.dropout(leaf, 0.5, key),
+                  ops.residual_norm(leaf, pre_weight=v)[1]):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, d)

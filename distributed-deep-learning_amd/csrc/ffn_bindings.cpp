@@ -8,7 +8,9 @@
 #include "ddl_kernels.h"
 #include "ffn_common.h"
 #include "ffn_misc.h"
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <limits>
 
 namespace {
@@ -43,6 +45,14 @@ void no_tangent(const Tensor& t, const char* op) {
 }
 void no_tangents(std::initializer_list<const Tensor*> ts, const char* op) {
   for (const Tensor* t : ts) no_tangent(*t, op);
+}
+
+// torch.jit.trace and make_fx record what goes through PyTorch's dispatcher; these calls do not.  A recorded program would hold this
+// call's result as a constant, so a call is refused while either records.
+void not_recorded(const char* op) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() &&
+                                  !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+                              op, ": cannot be recorded by torch.jit.trace or make_fx");
 }
 
 // `t` may stand beside `x` in a call: same device and type
@@ -232,6 +242,7 @@ Tensor product_forward(const Tensor& x, const Tensor& w0, const Tensor& w1, cons
 struct ProductGrads { Tensor dx, dw[2], db[2]; };
 ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width, int act, bool need_dx, bool need_dw, bool need_db,
                               const char* op) {
+  not_recorded(op);
   const Tensor &x = kept.x, &w0 = kept.w[0], &w1 = kept.w[1], &z = kept.z;
   const int dtype = type_of(x, op);
   const Tensor x2 = rows_of(x), dy2 = rows_of(dy);
@@ -363,6 +374,7 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
 // what linear checks; then the pieces that the model's units call: forward -> (y, z), backward -> (dx, dw, db)
 void check_linear(const Tensor& x, const Tensor& w, const OptT& b, const OptT& res, int64_t act) {
   const Tensor bias = get(b), residual = get(res);
+  not_recorded("linear");
   no_tangents({&x, &w, &bias, &residual}, "linear");
   check_product(x, w, b, "linear", "weight", "bias");
   check_act(act, "linear");
@@ -458,6 +470,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const OptT& b, const OptT& res, 
 
 void check_gated(const Tensor& x, const Tensor& wg, const Tensor& wu, const OptT& bg, const OptT& bu, int64_t act) {
   const Tensor b0 = get(bg), b1 = get(bu);
+  not_recorded("gated_linear");
   no_tangents({&x, &wg, &wu, &b0, &b1}, "gated_linear");
   check_product(x, wg, bg, "gated_linear", "w_gate", "b_gate");
   check_product(x, wu, bu, "gated_linear", "w_up", "b_up");
@@ -523,6 +536,7 @@ Tensor gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu, const O
 
 // ---- dropout ------------------------------------------------------------------------------------------------------------
 void check_dropout(const Tensor& x, double p, const Tensor& key, const OptT& res) {
+  not_recorded("dropout");
   no_tangent(x, "dropout");
   no_tangent(get(res), "dropout");
   BAD_UNLESS(x.is_cuda(), "dropout: GPU tensor expected");
@@ -579,6 +593,7 @@ Tensor dropout(const Tensor& x, double p, const Tensor& key, const OptT& res) {
   return dropout_apply(x, p, key, res);
 }
 Tensor rng_keys(Tensor state, int64_t n) {
+  not_recorded("rng_keys");
   DDL_CHECK_DEV(state); DDL_CHECK_CONTIG(state);
   BAD_UNLESS(state.scalar_type() == at::kLong && state.numel() == 2, "rng_keys: state must be two int64 values");
   BAD_UNLESS(n >= 1 && n <= (1 << 20), "rng_keys: 1 .. 2^20 keys, got ", n);
@@ -597,6 +612,7 @@ struct NormIn {
 struct NormSetup { ffn::NormArgs a; Tensor keep[8]; int dtype = 0; };
 NormSetup norm_setup(const NormIn& in) {
   const char* op = "residual_norm";
+  not_recorded(op);
   no_tangents({&in.x, &in.y, &in.gate, &in.post_w, &in.post_b, &in.pre_w, &in.pre_b}, op);
   BAD_UNLESS(in.x.is_cuda(), op, ": GPU tensor expected");
   NormSetup s;

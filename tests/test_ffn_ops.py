@@ -131,3 +131,22 @@ def test_forward_mode_is_right_or_refused():
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
                 pytest.fail(f"call {i} was not refused")
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_recorded_programs_are_right_or_refused():
+    """The plain path can be recorded; a kernel's result would be recorded as a constant, so its call refuses, before anything else."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, v, key = rnd(torch.float32, 4, 8, seed=1), rnd(torch.float32, 8, 8, seed=2), torch.ones(8), torch.tensor([1, 2])
+    other = rnd(torch.float32, 4, 8, seed=3)
+    for record in (lambda f: torch.jit.trace(f, (x,), check_trace=False), lambda f: make_fx(f)(x)):
+        plain = record(lambda t: ops.linear(t, w, activation="silu"))
+        assert torch.equal(plain(other), ops.linear(other, w, activation="silu"))
+        ext = ops.load_ext()
+        if ext is None:
+            pytest.skip("extension not built")
+        for call in (lambda t: ext.linear(t, w, None, None, 0), lambda t: ext.gated_linear(t, w, w, None, None, 2),
+                     lambda t: ext.dropout(t, 0.5, key, None), lambda t: ext.rng_keys(key, 1),
+                     lambda t: ext.residual_norm(t, None, None, None, None, v, None, False, 1e-6, 1.0)[1]):
+            with pytest.raises(NotImplementedError, match="recorded"):
+                record(call)

@@ -11,7 +11,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/jit/frontend/tracer.h>
-#include <limits>
+#include <string>
 
 namespace {
 
@@ -166,6 +166,38 @@ std::vector<int64_t> out_sizes(const Tensor& x, int64_t n) {
   return s;
 }
 
+// The three products of [M, K] x [N, K]^T as the kernels see them
+ffn::GemmArgs forward_shape(int M, int K, int N, bool dual) {
+  ffn::GemmArgs g;
+  g.N = N; g.M = M; g.K = K;
+  g.dual = dual;
+  return g;
+}
+ffn::GemmArgs dx_shape(int M, int K, int N, int weights) {           // dx[m][k] = sum over weights, n of dz[m][n] w[n][k]
+  ffn::GemmArgs g;
+  g.N = K; g.M = M; g.K = N;
+  g.nseg = weights;
+  g.p_kc = false;
+  return g;
+}
+ffn::GemmArgs dw_shape(int M, int K, int N, int weights) {           // dw[n][k] = sum over m of dz[m][n] x[m][k]
+  ffn::GemmArgs g;
+  g.N = K; g.M = N; g.K = M;
+  g.nout = weights;
+  g.p_kc = g.q_kc = false;
+  return g;
+}
+// -> rows and columns of the tile, splits: what the cost rule gives a product of more than FEW_ROWS rows (host only)
+std::tuple<int, int, int> product_plan(const std::string& what, const std::string& type, int64_t M, int64_t K, int64_t N, bool dual) {
+  BAD_UNLESS(what == "forward" || what == "dx" || what == "dw", "product_plan: forward, dx or dw expected, got ", what);
+  BAD_UNLESS(type == "fp32" || type == "bf16" || type == "fp16", "product_plan: fp32, bf16 or fp16 expected, got ", type);
+  const int m = dim_of(M, "product_plan"), k = dim_of(K, "product_plan"), n = dim_of(N, "product_plan"), weights = dual ? 2 : 1;
+  const ffn::GemmArgs g = what == "forward" ? forward_shape(m, k, n, dual) : what == "dx" ? dx_shape(m, k, n, weights)
+                                                                                         : dw_shape(m, k, n, weights);
+  const ffn::GemmPlan plan = ffn::gemm_plan(type == "fp32" ? ffn::F32 : type == "bf16" ? ffn::BF16 : ffn::F16, g);
+  return {plan.bm, plan.bn, plan.splits};
+}
+
 // What a product keeps for its backward pass: the fp32 sums z (one or two planes [M, ldz]; none without an activation), and x and the
 // weights as they were packed (otherwise as given).
 struct Kept { Tensor z, x, w[2]; };
@@ -227,9 +259,7 @@ Tensor product_forward(const Tensor& x, const Tensor& w0, const Tensor& w1, cons
     if (wo.keep.size(1) != K) kept->w[0] = wo.keep;
     if (dual && vo.keep.size(1) != K) kept->w[1] = vo.keep;
   }
-  ffn::GemmArgs g;
-  g.N = N; g.M = M; g.K = K;
-  g.dual = dual;
+  ffn::GemmArgs g = forward_shape(M, K, N, dual);
   g.p[0] = wo.p; g.ldp[0] = wo.ld;
   g.p[1] = vo.p; g.ldp[1] = vo.ld;
   g.q[0] = xo.p; g.ldq[0] = xo.ld;
@@ -318,12 +348,9 @@ ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width,
     }
   }
   if (K == 0) return r;
-  if (need_dx) {                                                     // dx[m][k] = sum over weights, n of dz[m][n] w[n][k]
-    ffn::GemmArgs g;
-    g.N = K; g.M = R; g.K = N;
+  if (need_dx) {
+    ffn::GemmArgs g = dx_shape(R, K, N, D);
     g.halves = two;
-    g.nseg = D;
-    g.p_kc = false;
     for (int d = 0; d < D; ++d) {
       g.p[d] = wo[d].p; g.ldp[d] = wo[d].ld;
       g.q[d] = dzo[d].p; g.ldq[d] = dzo[d].ld;
@@ -346,11 +373,8 @@ ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width,
       o.out[d] = r.dw[d].data_ptr();
     }
     ffn::launch_outer(dtype, o, cur_stream());
-  } else if (need_dw) {                                              // dw[n][k] = sum over m of dz[m][n] x[m][k]
-    ffn::GemmArgs g;
-    g.N = K; g.M = N; g.K = M;
-    g.nout = D;
-    g.p_kc = g.q_kc = false;
+  } else if (need_dw) {
+    ffn::GemmArgs g = dw_shape(M, K, N, D);
     g.p[0] = xo.p; g.ldp[0] = xo.ld;
     for (int d = 0; d < D; ++d) {
       g.q[d] = dzo[d].p; g.ldq[d] = dzo[d].ld;
@@ -824,6 +848,7 @@ void register_ffn_ops(pybind11::module_& m) {
   m.def("linear", &linear);
   m.def("linear_forward", &linear_forward, "-> (y, kept sums)");
   m.def("linear_backward", &linear_backward, "-> (dx, dweight, dbias)");
+  m.def("product_plan", &product_plan, "(forward | dx | dw, type, M, K, N, dual) -> (tile rows, tile columns, splits)");
   m.def("gated_linear", &gated_linear);
   m.def("gated_forward", &gated_forward, "-> (h, kept sums)");
   m.def("gated_backward", &gated_backward, "-> (dx, dw_gate, dw_up, db_gate, db_up)");

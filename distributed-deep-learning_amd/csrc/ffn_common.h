@@ -181,8 +181,8 @@ struct GemmArgs {
   Epilogue ep;
 };
 enum Tile : int { TILE_128x32 = 0, TILE_64x32 = 1, TILE_64x64 = 2, TILE_128x128 = 3, TILE_256x128 = 4, TILE_256x256 = 5, N_TILES = 6 };
-// bytes of `partial` the launch needs with the split it would choose (0: none)
-struct GemmPlan { int cfg = 0, splits = 1; long ldw = 0; long partial_floats = 0; };
+// Tile (rows and columns of the output) and split of a launch; partial_floats: the floats `partial` needs with that split (0: none)
+struct GemmPlan { int cfg = 0, splits = 1, bm = 0, bn = 0; long ldw = 0; long partial_floats = 0; };
 GemmPlan gemm_plan(int dtype, const GemmArgs& a);
 void launch_gemm(int dtype, GemmArgs a, const GemmPlan& plan, hipStream_t s);      // + the joining launch if split
 void launch_gemm_f32(const GemmArgs& a, int cfg, hipStream_t s);

@@ -271,6 +271,8 @@ GemmPlan gemm_plan(int dtype, const GemmArgs& a) {
       if (us < best_us) {
         best_us = us;
         best.cfg = cfg;
+        best.bm = c.bm;
+        best.bn = width;
         best.splits = (int)splits;
         best.partial_floats = join ? (long)floats : 0;
       }

@@ -150,3 +150,17 @@ def test_recorded_programs_are_right_or_refused():
                      lambda t: ext.residual_norm(t, None, None, None, None, v, None, False, 1e-6, 1.0)[1]):
             with pytest.raises(NotImplementedError, match="recorded"):
                 record(call)
+
+
+def test_plans_of_the_large_products():
+    """tests/test_gpu_ffn_edges.py reaches the large tiles through these sizes: the cost rule still gives them."""
+    from test_gpu_ffn_edges import LARGE
+    ext = ops.load_ext()
+    if ext is None:
+        pytest.skip("extension not built")
+    for (gated, M, K, N), plans in LARGE.items():
+        for name in ("bf16", "fp16"):
+            assert [ext.product_plan(what, name, M, K, N, gated) for what in ("forward", "dx", "dw")] == plans, (gated, M, K, N)
+    for bad in (("back", "bf16"), ("dx", "int8")):
+        with pytest.raises(ValueError):
+            ext.product_plan(*bad, 64, 64, 64, False)

@@ -4,8 +4,7 @@ in an unusual layout, the explicit forward / backward pairs, sizes at the limits
 import pytest
 import torch
 
-import ffn_oracle as oracle
-from test_gpu_ffn import EPS, IDS, TYPES, check_gated, check_linear, close, rnd
+from test_gpu_ffn import IDS, TYPES, check_gated, check_linear, product_bounds, rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +99,58 @@ def test_dual_tensors_are_refused(dev):
                   ops.residual_norm(leaf, pre_weight=v)[1]):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 torch.autograd.grad(y, leaf, d)
+
+
+# ---- large tiles, values -----------------------------------------------------------------------------------------------------
+# (gated, M, K, N) -> (tile rows, tile columns, splits) of the forward product, d_x and d_w in 16 bits.  Together: both large tiles as
+# single and as dual products, with one and two contraction segments, split and whole, with k starting elsewhere on each XCD (sizes of
+# whole tiles and slabs), with tiles moved back inside off every vector (N % 8 = 4, odd), and slabs that end inside.
+LARGE = {
+    (False, 2560, 4096, 2816): [(128, 256, 1), (256, 256, 1), (256, 256, 1)],
+    (False, 2100, 2048, 4200): [(256, 256, 1), (128, 256, 1), (256, 256, 1)],
+    (False, 2500, 2500, 2501): [(128, 256, 1), (128, 256, 1), (128, 256, 1)],
+    (False, 3001, 2052, 2052): [(128, 256, 1), (128, 256, 1), (128, 256, 1)],
+    (False, 4001, 200, 3977): [(256, 256, 1), (32, 128, 1), (32, 128, 1)],
+    (False, 4001, 200, 3980): [(256, 256, 1), (32, 128, 1), (32, 128, 1)],
+    (True, 2048, 1024, 4096): [(256, 128, 1), (128, 256, 4), (128, 256, 1)],
+    (True, 2011, 1000, 2708): [(256, 128, 1), (128, 256, 4), (128, 256, 1)],
+    (True, 1500, 1030, 2300): [(128, 128, 1), (128, 256, 4), (128, 256, 1)],
+    (True, 2051, 1100, 2051): [(256, 128, 1), (128, 256, 2), (128, 256, 1)],
+    (True, 2560, 2048, 2560): [(256, 128, 1), (128, 256, 1), (256, 256, 1)],
+    (True, 2500, 2052, 2052): [(256, 128, 1), (128, 256, 1), (256, 256, 1)],
+}
+
+
+def check_kept_sums(dev, ext, dtype, gated, M, K, N, bias):
+    """What the forward pass keeps: the fp32 sums themselves, element for element."""
+    x, b = rnd(dev, dtype, M, K, seed=1), rnd(dev, dtype, N, seed=4) if bias else None
+    w = [rnd(dev, dtype, N, K, seed=2 + i, scale=K ** -0.5) for i in range(1 + gated)]
+    z = (ext.gated_forward(x, *w, b, b, 2, True) if gated else ext.linear_forward(x, *w, b, None, 2, True))[1]
+    assert z.shape[:2] == (1 + gated, M) and z.dtype == torch.float32
+    for plane, v in zip(z, w):
+        want, bound = product_bounds(x.double(), v.double(), b.double() if bias else None, "silu")
+        assert ((plane[:, :N].double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("case", list(LARGE), ids=str)
+def test_large_tiles(dev, ext, dtype, case):
+    gated, M, K, N = case
+    name = "bf16" if dtype == torch.bfloat16 else "fp16"
+    assert [ext.product_plan(what, name, M, K, N, gated) for what in ("forward", "dx", "dw")] == LARGE[case]
+    bias = N % 3 > 0
+    check_kept_sums(dev, ext, dtype, gated, M, K, N, bias)
+    x, w = rnd(dev, dtype, M, K, seed=1), [rnd(dev, dtype, N, K, seed=2 + i, scale=K ** -0.5) for i in range(1 + gated)]
+    b = [rnd(dev, dtype, N, seed=4 + i) if bias else None for i in range(1 + gated)]
+    if gated:
+        check_gated(dev, dtype, x, *w, *b, "gelu")
+    else:
+        check_linear(dev, dtype, x, *w, *b, "gelu", rnd(dev, dtype, M, N, seed=6))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("gated", [False, True], ids=["linear", "gated"])
+@pytest.mark.parametrize("M,K,N", [(5, 40, 19), (70, 41, 23), (300, 200, 260), (900, 300, 1203), (1500, 200, 2052),
+                                   (2049, 100, 4101)])
+def test_kept_sums(dev, ext, dtype, gated, M, K, N):
+    check_kept_sums(dev, ext, dtype, gated, M, K, N, bias=True)

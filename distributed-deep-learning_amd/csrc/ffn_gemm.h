@@ -182,11 +182,20 @@ __device__ __forceinline__ void tile_of(int id, int tn, int tm, int& nt, int& mt
   nt = in / gm;
 }
 
+// What lanes of this wave wrote to LDS before is what its other lanes read behind.  LDS serves a wave in order, so this costs no
+// instruction: it keeps the compiler from moving one lane's read in front of another's write, of which it cannot know.
+__device__ __forceinline__ void wave_meet() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Results of a wave: lane holds rows 4 kg + r of each MFMA tile, i.e. V consecutive columns of the output for every tile (fp32) or pair
 // of tiles (16 bits), and column i (a row of the output).  Dual products: the upper half of the tiles belongs to the second weight.
 // CHUNK > 0: the sums go through LDS, CHUNK of the wave's row tiles at a time, so that one piece of code serves them in a loop: unrolled over
 // all of them with the activations inside, it outgrows the instruction cache, and a tile waits for its code (8192 x 4096 x 4096 bf16 with
-// gelu and residual: 285 us unrolled, 252 so).  The ring is no longer read then; `lds` is this wave's part, and each lane reads back what it wrote.
+// gelu and residual: 285 us unrolled, 252 so).  The ring is no longer read then; `lds` is this wave's part: each lane reads back what it
+// wrote, and where the kept sums of a dual product are stored by rows, what other lanes of the wave wrote.
 template <typename T, typename P, typename Q, bool PKC, bool QKC, bool DUAL, int NT, int MT, int CHUNK>
 __device__ __forceinline__ void finish(const GemmArgs& a, const f32x4 (&acc)[NT][MT], int n0, int pw0, int m0, int qw0, int which,
                                        int split, char* lds) {
@@ -256,6 +265,7 @@ __device__ __forceinline__ void finish(const GemmArgs& a, const f32x4 (&acc)[NT]
       for (int u = 0; u < CHUNK; ++u)
 #pragma unroll
         for (int t = 0; t < NT; ++t) mine[(u * NT + t) * 64] = acc[t][u0 + u];
+      wave_meet();
 #pragma unroll 1
       for (int u = 0; u < CHUNK; ++u) {
         if (keep) {
@@ -273,6 +283,7 @@ __device__ __forceinline__ void finish(const GemmArgs& a, const f32x4 (&acc)[NT]
         for (int t = 0; t < NT; ++t) sums[t] = mine[(u * NT + t) * 64];
         row(m0 + Q::row_of(qw0, u0 + u, i), sums);
       }
+      wave_meet();                                         // the next chunk is written where this one was read
     }
   }
 }

@@ -633,49 +633,32 @@ struct NormIn {
   bool layer = false;
   double eps = 0., scale = 1.;
 };
-struct NormSetup { ffn::NormArgs a; Tensor keep[8]; int dtype = 0; };
-NormSetup norm_setup(const NormIn& in) {
+bool full_gate(const NormIn& in) { return in.gate.defined() && !(in.gate.dim() == 1 && in.x.dim() != 1); }
+// The checks alone: nothing is copied or launched.
+void check_norm(const NormIn& in) {
   const char* op = "residual_norm";
   not_recorded(op);
   no_tangents({&in.x, &in.y, &in.gate, &in.post_w, &in.post_b, &in.pre_w, &in.pre_b}, op);
   BAD_UNLESS(in.x.is_cuda(), op, ": GPU tensor expected");
-  NormSetup s;
-  s.dtype = type_of(in.x, op);
+  type_of(in.x, op);
   BAD_UNLESS(in.x.dim() >= 1 && in.x.size(-1) >= 1, op, ": x [.., C] with C >= 1 expected, got ", in.x.sizes());
   const int64_t C = in.x.size(-1);
   BAD_UNLESS(C <= ffn::NORM_MAX_C, op, ": rows of at most ", ffn::NORM_MAX_C, " columns, got ", C);
+  dim_of(in.x.numel() / C, op);
   BAD_UNLESS(in.eps >= 0., op, ": eps must not be negative");
-  const bool layer = in.layer;
-  BAD_UNLESS(layer || !(in.post_b.defined() || in.pre_b.defined()), op, ": an RMS norm has no bias");
+  BAD_UNLESS(in.layer || !(in.post_b.defined() || in.pre_b.defined()), op, ": an RMS norm has no bias");
   BAD_UNLESS(in.post_w.defined() || !in.post_b.defined(), op, ": post_bias without post_weight");
   BAD_UNLESS(in.pre_w.defined() || !in.pre_b.defined(), op, ": pre_bias without pre_weight");
   BAD_UNLESS(in.y.defined() || !(in.gate.defined() || in.post_w.defined()), op, ": gate or post_weight without a branch");
   BAD_UNLESS(in.y.defined() || in.pre_w.defined(), op, ": neither a branch nor pre_weight: nothing to do");
-  ffn::NormArgs& a = s.a;
-  a.C = (int)C;
-  a.M = dim_of(in.x.numel() / C, op);
-  a.layer = layer;
-  a.eps = (float)in.eps;
-  a.scale = (float)in.scale;
-  a.post = in.post_w.defined();
-  a.pre = in.pre_w.defined();
-  bool vec = C * in.x.element_size() % 16 == 0;
-  auto rows = [&](const Tensor& t, int i) -> const void* {
-    if (!t.defined()) return nullptr;
-    s.keep[i] = t.contiguous();
-    vec = vec && aligned(s.keep[i].data_ptr());
-    return s.keep[i].data_ptr();
-  };
   if (in.y.defined()) {
     check_like(in.y, in.x, op, "the branch");
     BAD_UNLESS(in.y.sizes() == in.x.sizes(), op, ": branch ", in.y.sizes(), " where x is ", in.x.sizes());
   }
-  a.x = rows(in.x, 0);
-  a.y = rows(in.y, 1);
   at::ScalarType pt = in.x.scalar_type();
   bool first = true;
-  auto param = [&](const Tensor& t, int i, const char* name) -> const void* {
-    if (!t.defined()) return nullptr;
+  auto param = [&](const Tensor& t, const char* name) {
+    if (!t.defined()) return;
     BAD_UNLESS(t.dim() == 1 && t.size(0) == C, op, ": ", name, " [", C, "] expected, got ", t.sizes());
     BAD_UNLESS(t.device() == in.x.device(), op, ": ", name, " is on another device");
     BAD_UNLESS(t.scalar_type() == in.x.scalar_type() || t.scalar_type() == at::kFloat, op, ": ", name, " must be float32 or ",
@@ -683,33 +666,53 @@ NormSetup norm_setup(const NormIn& in) {
     BAD_UNLESS(first || t.scalar_type() == pt, op, ": weights, biases and a channel gate share one type");
     pt = t.scalar_type();
     first = false;
-    return rows(t, i);
   };
-  a.post_w = param(in.post_w, 2, "post_weight");
-  a.post_b = param(in.post_b, 3, "post_bias");
-  a.pre_w = param(in.pre_w, 4, "pre_weight");
-  a.pre_b = param(in.pre_b, 5, "pre_bias");
-  if (in.gate.defined()) {
-    if (in.gate.dim() == 1 && in.x.dim() != 1) {
-      a.gate_kind = ffn::GATE_CHANNEL;
-      a.gate = param(in.gate, 6, "gate");
-    } else {
-      check_like(in.gate, in.x, op, "a gate of x's shape");
-      BAD_UNLESS(in.gate.sizes() == in.x.sizes(), op, ": gate [", C, "] or of x's shape ", in.x.sizes(), " expected, got ",
-                 in.gate.sizes());
-      a.gate_kind = ffn::GATE_FULL;
-      a.gate = rows(in.gate, 6);
-    }
+  param(in.post_w, "post_weight");
+  param(in.post_b, "post_bias");
+  param(in.pre_w, "pre_weight");
+  param(in.pre_b, "pre_bias");
+  if (full_gate(in)) {
+    check_like(in.gate, in.x, op, "a gate of x's shape");
+    BAD_UNLESS(in.gate.sizes() == in.x.sizes(), op, ": gate [", C, "] or of x's shape ", in.x.sizes(), " expected, got ",
+               in.gate.sizes());
+  } else {
+    param(in.gate, "gate");
   }
+}
+// The inputs as the kernels read them: rows behind each other.  The backward pass keeps these, so a strided input is copied once.
+NormIn contiguous(const NormIn& in) {
+  NormIn c = in;
+  for (Tensor* t : {&c.x, &c.y, &c.gate, &c.post_w, &c.post_b, &c.pre_w, &c.pre_b})
+    if (t->defined()) *t = t->contiguous();
+  return c;
+}
+// of checked, contiguous inputs
+ffn::NormArgs norm_args(const NormIn& in) {
+  ffn::NormArgs a;
+  a.C = (int)in.x.size(-1);
+  a.M = (int)(in.x.numel() / a.C);
+  a.layer = in.layer;
+  a.eps = (float)in.eps;
+  a.scale = (float)in.scale;
+  a.post = in.post_w.defined();
+  a.pre = in.pre_w.defined();
+  a.gate_kind = !in.gate.defined() ? ffn::GATE_NONE : full_gate(in) ? ffn::GATE_FULL : ffn::GATE_CHANNEL;
+  at::ScalarType pt = in.x.scalar_type();
+  for (const Tensor* t : {&in.post_w, &in.pre_w, &in.gate})          // all vectors have one type
+    if (t->defined() && !(t == &in.gate && full_gate(in))) pt = t->scalar_type();
   a.param_f32 = pt == at::kFloat;
-  a.vec = vec;
-  return s;
+  a.x = ptr(in.x); a.y = ptr(in.y); a.gate = ptr(in.gate);
+  a.post_w = ptr(in.post_w); a.post_b = ptr(in.post_b);
+  a.pre_w = ptr(in.pre_w); a.pre_b = ptr(in.pre_b);
+  a.vec = a.C * in.x.element_size() % 16 == 0;
+  for (const void* p : {a.x, a.y, a.gate, a.post_w, a.post_b, a.pre_w, a.pre_b}) a.vec = a.vec && aligned(p);
+  return a;
 }
 // -> r (undefined without a branch), h (undefined without a pre norm), statistics [4, M] if `keep`
+// (checked, contiguous inputs)
 std::tuple<Tensor, Tensor, Tensor> norm_forward(const NormIn& in, bool keep) {
-  NormSetup s = norm_setup(in);
   ddl::DeviceGuard guard(in.x.device());
-  ffn::NormArgs& a = s.a;
+  ffn::NormArgs a = norm_args(in);
   Tensor r, h, st;
   if (in.y.defined()) r = at::empty(in.x.sizes(), in.x.options());
   if (a.pre) h = at::empty(in.x.sizes(), in.x.options());
@@ -717,15 +720,15 @@ std::tuple<Tensor, Tensor, Tensor> norm_forward(const NormIn& in, bool keep) {
   a.r = r.defined() ? r.data_ptr() : nullptr;
   a.h = h.defined() ? h.data_ptr() : nullptr;
   a.stats = keep ? st.data_ptr<float>() : nullptr;
-  if (a.M > 0) ffn::launch_norm_fwd(s.dtype, a, cur_stream());
+  if (a.M > 0) ffn::launch_norm_fwd(type_of(in.x, "residual_norm"), a, cur_stream());
   return {r, h, st};
 }
 struct NormGrads { Tensor dx, dy, v[5]; };                           // v: gate, post_w, post_b, pre_w, pre_b
 NormGrads norm_backward(const NormIn& in, const Tensor& st, const Tensor& dr, const Tensor& dh, bool need_dx, bool need_dy,
                         bool need_gate, bool need_post_w, bool need_post_b, bool need_pre_w, bool need_pre_b) {
-  NormSetup s = norm_setup(in);
   ddl::DeviceGuard guard(in.x.device());
-  ffn::NormArgs& a = s.a;
+  ffn::NormArgs a = norm_args(in);
+  const int dtype = type_of(in.x, "residual_norm");
   NormGrads g;
   BAD_UNLESS(st.defined() && st.is_contiguous() && st.scalar_type() == at::kFloat && st.numel() == 4 * (int64_t)a.M &&
                  st.device() == in.x.device(), "residual_norm: the backward pass needs the statistics kept by the forward pass");
@@ -771,8 +774,8 @@ NormGrads norm_backward(const NormIn& in, const Tensor& st, const Tensor& dr, co
     means = at::empty({2, a.M}, in.x.options().dtype(at::kFloat));
     a.means = means.data_ptr<float>();
   }
-  ffn::launch_norm_bwd(s.dtype, a, cur_stream());
-  if (any) ffn::launch_colsum(a.param_f32 ? (int)ffn::F32 : s.dtype, a.part, a.groups, 5, a.C, outs, cur_stream());
+  ffn::launch_norm_bwd(dtype, a, cur_stream());
+  if (any) ffn::launch_colsum(a.param_f32 ? (int)ffn::F32 : dtype, a.part, a.groups, 5, a.C, outs, cur_stream());
   return g;
 }
 NormIn norm_in(const Tensor& x, const OptT& y, const OptT& gate, const OptT& post_w, const OptT& post_b, const OptT& pre_w,
@@ -791,9 +794,9 @@ struct NormFn : torch::autograd::Function<NormFn> {
                                const OptT& post_b, const OptT& pre_w, const OptT& pre_b, bool layer, double eps, double scale) {
     at::AutoDispatchBelowADInplaceOrView below;
     Needs::remember(ctx, {true, has(y), has(gate), has(post_w), has(post_b), has(pre_w), has(pre_b)});
-    const NormIn in = norm_in(x, y, gate, post_w, post_b, pre_w, pre_b, layer, eps, scale);
+    const NormIn in = contiguous(norm_in(x, y, gate, post_w, post_b, pre_w, pre_b, layer, eps, scale));
     auto [r, h, st] = norm_forward(in, true);
-    ctx->save_for_backward({x, in.y, in.gate, in.post_w, in.post_b, in.pre_w, in.pre_b, st});
+    ctx->save_for_backward({in.x, in.y, in.gate, in.post_w, in.post_b, in.pre_w, in.pre_b, st});
     ctx->saved_data["layer"] = layer;
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["scale"] = scale;
@@ -805,6 +808,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_second_derivative("residual_norm");
+    not_recorded("residual_norm");
     const auto v = ctx->get_saved_variables();
     const NormIn in = norm_in(v[0], v[1], v[2], v[3], v[4], v[5], v[6], ctx->saved_data["layer"].toBool(),
                               ctx->saved_data["eps"].toDouble(), ctx->saved_data["scale"].toDouble());
@@ -829,15 +833,16 @@ struct NormFn : torch::autograd::Function<NormFn> {
 std::tuple<Tensor, OptT> residual_norm(const Tensor& x, const OptT& y, const OptT& gate, const OptT& post_w, const OptT& post_b,
                                        const OptT& pre_w, const OptT& pre_b, bool layer, double eps, double scale) {
   const NormIn in = norm_in(x, y, gate, post_w, post_b, pre_w, pre_b, layer, eps, scale);
+  check_norm(in);
+  ddl::DeviceGuard guard(x.device());
   Tensor r, h;
   if (wants_grad({&in.x, &in.y, &in.gate, &in.post_w, &in.post_b, &in.pre_w, &in.pre_b})) {
-    norm_setup(in);
     auto out = NormFn::apply(x, y, gate, post_w, post_b, pre_w, pre_b, layer, eps, scale);
     size_t i = 0;
     if (in.y.defined()) r = out[i++];
     if (in.pre_w.defined()) h = out[i];
   } else {
-    std::tie(r, h, std::ignore) = norm_forward(in, false);
+    std::tie(r, h, std::ignore) = norm_forward(contiguous(in), false);
   }
   return {r.defined() ? r : x, h.defined() ? OptT(h) : OptT()};
 }
@@ -857,12 +862,17 @@ void register_ffn_ops(pybind11::module_& m) {
   m.def("residual_norm", &residual_norm);
   m.def("norm_forward", [](const Tensor& x, const OptT& y, const OptT& gate, const OptT& post_w, const OptT& post_b, const OptT& pre_w,
                            const OptT& pre_b, bool layer, double eps, double scale) {
-    return norm_forward(norm_in(x, y, gate, post_w, post_b, pre_w, pre_b, layer, eps, scale), true);
+    const NormIn in = norm_in(x, y, gate, post_w, post_b, pre_w, pre_b, layer, eps, scale);
+    check_norm(in);
+    ddl::DeviceGuard guard(x.device());
+    return norm_forward(contiguous(in), true);
   }, "-> (r, h, statistics)");
   m.def("norm_backward", [](const Tensor& x, const OptT& y, const OptT& gate, const OptT& post_w, const OptT& post_b, const OptT& pre_w,
                             const OptT& pre_b, bool layer, double eps, double scale, const Tensor& stats, const OptT& dr, const OptT& dh) {
     const NormIn in = norm_in(x, y, gate, post_w, post_b, pre_w, pre_b, layer, eps, scale);
-    NormGrads g = norm_backward(in, stats, get(dr), get(dh), true, has(y), has(gate), has(post_w), has(post_b), has(pre_w), has(pre_b));
+    check_norm(in);
+    ddl::DeviceGuard guard(x.device());
+    NormGrads g = norm_backward(contiguous(in), stats, get(dr), get(dh), true, has(y), has(gate), has(post_w), has(post_b), has(pre_w), has(pre_b));
     return std::make_tuple(g.dx, g.dy, g.v[0], g.v[1], g.v[2], g.v[3], g.v[4]);
   }, "-> (dx, dbranch, dgate, dpost_w, dpost_b, dpre_w, dpre_b)");
 }

@@ -154,3 +154,26 @@ def test_large_tiles(dev, ext, dtype, case):
                                    (2049, 100, 4101)])
 def test_kept_sums(dev, ext, dtype, gated, M, K, N):
     check_kept_sums(dev, ext, dtype, gated, M, K, N, bias=True)
+
+
+# ---- residual_norm -----------------------------------------------------------------------------------------------------------
+def test_strided_norm_inputs_are_copied_once(dev):
+    """A step on strided rows makes one copy of each of them more than a step on contiguous rows, and gives the same bits."""
+    from ddl import ops
+    x, y, gate, dr, dh = (rnd(dev, torch.float32, 50, 64, seed=i) for i in range(5))
+    w = rnd(dev, torch.float32, 64, seed=6).requires_grad_(True)
+
+    def step(how):
+        leaves = [(strided(t, "transposed") if how else t.clone()).requires_grad_(True) for t in (x, y, gate)]
+        made = torch.cuda.memory_stats()["allocation.all.allocated"]
+        outs = ops.residual_norm(leaves[0], leaves[1], kind="layer", pre_weight=w, post_weight=w, gate=leaves[2])
+        grads = torch.autograd.grad(outs, leaves + [w], (dr, dh))
+        return torch.cuda.memory_stats()["allocation.all.allocated"] - made, [o.detach() for o in outs] + list(grads)
+
+    step(False)
+    plain, want = step(False)
+    copies, got = step(True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert copies - plain == 3
+    r, h = ops.residual_norm(strided(x, "transposed"), pre_weight=w.detach())
+    assert torch.equal(h, ops.residual_norm(x, pre_weight=w.detach())[1]) and not r.is_contiguous()

@@ -633,7 +633,10 @@ struct NormIn {
   bool layer = false;
   double eps = 0., scale = 1.;
 };
-bool full_gate(const NormIn& in) { return in.gate.defined() && !(in.gate.dim() == 1 && in.x.dim() != 1); }
+// Beside a single row [C] both kinds of gate have its shape: one of x's type is taken element by element, another is a channel gate.
+bool full_gate(const NormIn& in) {
+  return in.gate.defined() && (in.gate.dim() != 1 || (in.x.dim() == 1 && in.gate.scalar_type() == in.x.scalar_type()));
+}
 // The checks alone: nothing is copied or launched.
 void check_norm(const NormIn& in) {
   const char* op = "residual_norm";

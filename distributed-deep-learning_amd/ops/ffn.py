@@ -194,7 +194,7 @@ def residual_norm(x: torch.Tensor, branch: Optional[torch.Tensor] = None, kind: 
     _need(branch is not None or (gate is None and post_weight is None), "gate or post_weight without a branch")
     _need(branch is not None or pre_weight is not None, "neither a branch nor pre_weight: nothing to do")
     _like(branch, x, "branch", x.shape)
-    full = gate is not None and (gate.dim() != 1 or x.dim() == 1)
+    full = gate is not None and (gate.dim() != 1 or (x.dim() == 1 and gate.dtype == x.dtype))
     vectors = [v for v in (post_weight, post_bias, pre_weight, pre_bias, None if full else gate) if v is not None]
     for v in vectors:
         _need(tuple(v.shape) == (x.shape[-1],) and v.device == x.device, f"a vector [{x.shape[-1]}] expected, got {tuple(v.shape)}")

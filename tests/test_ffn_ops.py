@@ -164,3 +164,13 @@ def test_plans_of_the_large_products():
     for bad in (("back", "bf16"), ("dx", "int8")):
         with pytest.raises(ValueError):
             ext.product_plan(*bad, 64, 64, 64, False)
+
+
+def test_channel_gate_beside_a_single_row():
+    """A vector may be fp32 beside a 16-bit row, the gate of a single row [C] as well."""
+    for dtype in TYPES:
+        x, y, g, w = (rnd(t, 40, seed=i) for i, t in enumerate((dtype, dtype, torch.float32, torch.float32)))
+        got, want = ops.residual_norm(x, y, gate=g, pre_weight=w), ops.residual_norm(x[None], y[None], gate=g, pre_weight=w)
+        assert all(torch.equal(a, b[0]) for a, b in zip(got, want))
+    with pytest.raises(ValueError):                                  # vectors of two types
+        ops.residual_norm(x, y, gate=g, pre_weight=w.to(dtype))

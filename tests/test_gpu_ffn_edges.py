@@ -177,3 +177,17 @@ def test_strided_norm_inputs_are_copied_once(dev):
     assert copies - plain == 3
     r, h = ops.residual_norm(strided(x, "transposed"), pre_weight=w.detach())
     assert torch.equal(h, ops.residual_norm(x, pre_weight=w.detach())[1]) and not r.is_contiguous()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_channel_gate_beside_a_single_row(dev, dtype):
+    from ddl import ops
+    x, y, dr, dh = (rnd(dev, dtype, 72, seed=i) for i in range(4))
+    for ptype in {dtype, torch.float32}:
+        g, w = (rnd(dev, ptype, 72, seed=i).requires_grad_(True) for i in (5, 6))
+        X, Y = (t.clone().requires_grad_(True) for t in (x, y))
+        one = ops.residual_norm(X, Y, gate=g, pre_weight=w)
+        two = ops.residual_norm(X[None], Y[None], gate=g, pre_weight=w)
+        a = torch.autograd.grad(one, (X, Y, g, w), (dr, dh))
+        b = torch.autograd.grad(two, (X, Y, g, w), (dr[None], dh[None]))
+        assert all(torch.equal(p, q[0]) for p, q in zip(one, two)) and all(torch.equal(p, q) for p, q in zip(a, b))

@@ -60,8 +60,12 @@ void check_like(const Tensor& t, const Tensor& x, const char* op, const char* na
   BAD_UNLESS(t.device() == x.device(), op, ": ", name, " is on ", t.device(), ", the input on ", x.device());
   BAD_UNLESS(t.scalar_type() == x.scalar_type(), op, ": ", name, " is ", t.scalar_type(), ", the input ", x.scalar_type());
 }
-int dim_of(int64_t n, const char* op) {
-  BAD_UNLESS(n <= (1 << 30), op, ": at most 2^30 rows or columns, got ", n);
+int rows_fit(int64_t n, const char* op) {
+  BAD_UNLESS(n <= (1 << 30), op, ": at most 2^30 rows, got ", n);
+  return (int)n;
+}
+int width_fits(int64_t n, const char* op) {                          // a launch has fewer than 2^32 threads, up to 32 a column
+  BAD_UNLESS(n <= (1 << 26), op, ": rows of at most 2^26 columns, got ", n);
   return (int)n;
 }
 // [.., C] as [rows, C] whose columns are contiguous
@@ -136,6 +140,7 @@ void set_out(ffn::Epilogue& e, int i, const Tensor& out) {
 }
 void run_gemm(int dtype, ffn::GemmArgs& g, const Tensor& like) {
   const ffn::GemmPlan plan = ffn::gemm_plan(dtype, g);
+  BAD_UNLESS(plan.bm > 0, "a product of ", g.M, " x ", g.N, " results is more than one launch holds");
   Tensor ws;
   if (plan.partial_floats > 0) {
     ws = at::empty({plan.partial_floats}, like.options().dtype(at::kFloat));
@@ -191,7 +196,7 @@ ffn::GemmArgs dw_shape(int M, int K, int N, int weights) {           // dw[n][k]
 std::tuple<int, int, int> product_plan(const std::string& what, const std::string& type, int64_t M, int64_t K, int64_t N, bool dual) {
   BAD_UNLESS(what == "forward" || what == "dx" || what == "dw", "product_plan: forward, dx or dw expected, got ", what);
   BAD_UNLESS(type == "fp32" || type == "bf16" || type == "fp16", "product_plan: fp32, bf16 or fp16 expected, got ", type);
-  const int m = dim_of(M, "product_plan"), k = dim_of(K, "product_plan"), n = dim_of(N, "product_plan"), weights = dual ? 2 : 1;
+  const int m = rows_fit(M, "product_plan"), k = width_fits(K, "product_plan"), n = width_fits(N, "product_plan"), weights = dual ? 2 : 1;
   const ffn::GemmArgs g = what == "forward" ? forward_shape(m, k, n, dual) : what == "dx" ? dx_shape(m, k, n, weights)
                                                                                          : dw_shape(m, k, n, weights);
   const ffn::GemmPlan plan = ffn::gemm_plan(type == "fp32" ? ffn::F32 : type == "bf16" ? ffn::BF16 : ffn::F16, g);
@@ -207,7 +212,7 @@ Tensor product_forward(const Tensor& x, const Tensor& w0, const Tensor& w1, cons
                        int act, bool keep_sums, Kept* kept, const char* op) {
   const int dtype = type_of(x, op);
   const Tensor x2 = rows_of(x);
-  const int M = dim_of(x2.size(0), op), K = dim_of(x2.size(1), op), N = dim_of(w0.size(0), op);
+  const int M = rows_fit(x2.size(0), op), K = width_fits(x2.size(1), op), N = width_fits(w0.size(0), op);
   const bool dual = w1.defined();
   Tensor out = at::empty({M, N}, x.options()), z;
   if (keep_sums) z = at::empty({dual ? 2 : 1, M, up(N, 16)}, x.options().dtype(at::kFloat));
@@ -276,7 +281,7 @@ ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width,
   const Tensor &x = kept.x, &w0 = kept.w[0], &w1 = kept.w[1], &z = kept.z;
   const int dtype = type_of(x, op);
   const Tensor x2 = rows_of(x), dy2 = rows_of(dy);
-  const int M = dim_of(dy2.size(0), op), K = dim_of(width, op), N = dim_of(dy2.size(1), op);
+  const int M = rows_fit(dy2.size(0), op), K = width_fits(width, op), N = width_fits(dy2.size(1), op);
   const bool dual = w1.defined();
   const int D = dual ? 2 : 1;
   ProductGrads r;
@@ -647,7 +652,7 @@ void check_norm(const NormIn& in) {
   BAD_UNLESS(in.x.dim() >= 1 && in.x.size(-1) >= 1, op, ": x [.., C] with C >= 1 expected, got ", in.x.sizes());
   const int64_t C = in.x.size(-1);
   BAD_UNLESS(C <= ffn::NORM_MAX_C, op, ": rows of at most ", ffn::NORM_MAX_C, " columns, got ", C);
-  dim_of(in.x.numel() / C, op);
+  rows_fit(in.x.numel() / C, op);
   BAD_UNLESS(in.eps >= 0., op, ": eps must not be negative");
   BAD_UNLESS(in.layer || !(in.post_b.defined() || in.pre_b.defined()), op, ": an RMS norm has no bias");
   BAD_UNLESS(in.post_w.defined() || !in.post_b.defined(), op, ": post_bias without post_weight");

@@ -183,7 +183,7 @@ struct GemmArgs {
 enum Tile : int { TILE_128x32 = 0, TILE_64x32 = 1, TILE_64x64 = 2, TILE_128x128 = 3, TILE_256x128 = 4, TILE_256x256 = 5, N_TILES = 6 };
 // Tile (rows and columns of the output) and split of a launch; partial_floats: the floats `partial` needs with that split (0: none)
 struct GemmPlan { int cfg = 0, splits = 1, bm = 0, bn = 0; long ldw = 0; long partial_floats = 0; };
-GemmPlan gemm_plan(int dtype, const GemmArgs& a);
+GemmPlan gemm_plan(int dtype, const GemmArgs& a);                                   // bm == 0: no tile fits a launch
 void launch_gemm(int dtype, GemmArgs a, const GemmPlan& plan, hipStream_t s);      // + the joining launch if split
 void launch_gemm_f32(const GemmArgs& a, int cfg, hipStream_t s);
 void launch_gemm_bf16(const GemmArgs& a, int cfg, hipStream_t s);

@@ -26,6 +26,13 @@ namespace {
 // threads of a workgroup: four rows where a row is one wave (rows of more waves meet in barriers, so they have a workgroup each)
 constexpr int block_of(int tpr) { return tpr == 64 ? 256 : tpr; }
 
+// A launch has fewer than 2^32 threads along x, and a row has up to 1024: workgroup ids go on along y.
+__device__ __forceinline__ long group_id() { return (long)blockIdx.y * gridDim.x + blockIdx.x; }
+inline dim3 grid_of(long groups) {
+  const long y = (groups + 65535) / 65536;
+  return dim3((unsigned)((groups + y - 1) / y), (unsigned)y);
+}
+
 // The EL elements of a row that a thread holds: VEC: 16-byte chunks t, t + TPR, ...; otherwise single elements.
 template <typename T, int TPR, int EL, bool VEC> struct Row {
   static constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, NV = EL / V;
@@ -169,7 +176,7 @@ __global__ void __launch_bounds__(block_of(TPR)) norm_fwd_kernel(NormArgs a) {
   __shared__ float xbuf[2][16][2];
   Exchange red(xbuf);
   const int t = threadIdx.x % TPR, C = a.C;
-  const long m = (long)blockIdx.x * RPB + threadIdx.x / TPR;
+  const long m = group_id() * RPB + threadIdx.x / TPR;
   if (m >= a.M) return;                                    // whole waves (TPR = 64) or the whole workgroup
   float r[EL], n[EL], w[EL], hat[EL];
   R::template load<T>((const T*)a.x + m * C, t, C, r);
@@ -257,7 +264,7 @@ __global__ void __launch_bounds__(block_of(TPR)) norm_bwd_kernel(NormArgs a) {
     if (has_y && a.post) { st[0] = a.stats[m]; st[1] = a.stats[a.M + m]; }
     if (a.dh != nullptr) { st[2] = a.stats[2 * (long)a.M + m]; st[3] = a.stats[3 * (long)a.M + m]; }
   };
-  long m = (long)blockIdx.x * RPB + sub;
+  long m = group_id() * RPB + sub;
   if (SUMS && m < a.M) ahead(m);
   // a row group walks its rows; all threads of a row take the same turns (the row sums meet in barriers only if TPR > 64)
   for (; m < a.M; m += stride) {
@@ -481,7 +488,7 @@ template <typename F> void by_width(int C, bool forward, F f) {
 template <typename T> void fwd(const NormArgs& a, hipStream_t s) {
   by_width(a.C, true, [&](auto tpr, auto el) {
     constexpr int TPR = decltype(tpr)::value, EL = decltype(el)::value, RPB = block_of(TPR) / TPR;
-    const dim3 grid((a.M + RPB - 1) / RPB), block(block_of(TPR));
+    const dim3 grid = grid_of(((long)a.M + RPB - 1) / RPB), block(block_of(TPR));
     if (a.vec) hipLaunchKernelGGL((norm_fwd_kernel<T, TPR, EL, true>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((norm_fwd_kernel<T, TPR, EL, false>), grid, block, 0, s, a);
   });
@@ -490,7 +497,7 @@ template <typename T> void bwd(const NormArgs& a, hipStream_t s) {
   by_width(a.C, false, [&](auto tpr, auto el) {
     constexpr int TPR = decltype(tpr)::value, EL = decltype(el)::value;
     constexpr bool SUMS = TPR * EL <= SUMS_MAX_C;
-    const dim3 grid(SUMS ? a.groups : a.M), block(block_of(TPR));
+    const dim3 grid = SUMS ? dim3(a.groups) : grid_of(a.M), block(block_of(TPR));
     if (a.vec) hipLaunchKernelGGL((norm_bwd_kernel<T, TPR, EL, true, SUMS>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((norm_bwd_kernel<T, TPR, EL, false, SUMS>), grid, block, 0, s, a);
     if (!SUMS && a.part != nullptr) {

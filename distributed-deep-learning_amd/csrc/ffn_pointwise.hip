@@ -239,10 +239,11 @@ void launch_colsum(int out_dtype, const float* part, int chunks, int nvec, long 
 //   1500 x 5000 x 5000:  256 x 128 88 us, 256 x 256 122, 128 x 128 100;          8192 x 8192 x 8192: 256 x 256 first
 // A split writes its sums in fp32 and a second launch joins them: 3 us and the bytes at 2 TB/s.
 namespace {
-struct TileCost { int bn, bm; double one, two, end; };
-constexpr TileCost COST16[N_TILES] = {{128, 32, .30, .56, .4}, {64, 32, .22, .40, .5}, {64, 64, .30, .53, .4}, {128, 128, .80, 1.40, 1.},
-                                      {256, 128, 1.05, 2.1, 2.5}, {256, 256, 1.7, 3.4, 5.}};
-constexpr TileCost COST32[N_TILES] = {{128, 32, .71, 1.35, .6}, {64, 32, .42, .75, .6}, {64, 64, .66, 1.23, .7}, {128, 128, 2.4, 3.9, 2.}, {}, {}};
+struct TileCost { int bn, bm, threads; double one, two, end; };
+constexpr TileCost COST16[N_TILES] = {{128, 32, 512, .30, .56, .4}, {64, 32, 512, .22, .40, .5}, {64, 64, 512, .30, .53, .4},
+                                      {128, 128, 256, .80, 1.40, 1.}, {256, 128, 512, 1.05, 2.1, 2.5}, {256, 256, 512, 1.7, 3.4, 5.}};
+constexpr TileCost COST32[N_TILES] = {{128, 32, 512, .71, 1.35, .6}, {64, 32, 512, .42, .75, .6}, {64, 64, 512, .66, 1.23, .7},
+                                      {128, 128, 256, 2.4, 3.9, 2.}, {}, {}};
 }  // namespace
 
 GemmPlan gemm_plan(int dtype, const GemmArgs& a) {
@@ -259,6 +260,7 @@ GemmPlan gemm_plan(int dtype, const GemmArgs& a) {
     // k-strided 16-bit operands of 64 columns: every read of LDS is a transposing one, half as wide
     const double f = dtype != F32 && cfg == TILE_64x64 && !(a.p_kc && a.q_kc) ? 1.2 : 1.0;
     const long tiles = ((a.N + width - 1) / width) * (long)((a.M + c.bm - 1) / c.bm) * a.nout;
+    if (tiles * c.threads >= 1l << 32) continue;           // more threads than a launch may have
     for (long s = 1; s <= 32; s *= 2) {
       if (s > 1 && (s > slabs / 2 || tiles * s > 2048)) break;
       const long per = (slabs + s - 1) / s, splits = slabs > 0 ? (slabs + per - 1) / per : 1;      // no empty splits

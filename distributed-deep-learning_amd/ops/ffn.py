@@ -10,7 +10,7 @@ Together they are the residual block of a model's trunk or head::
 All four are differentiable once, by a backward pass (forward-mode tangents are refused on the GPU), take float32, bfloat16 and float16 (one type per call; the vectors of ``residual_norm`` may be
 float32 beside 16-bit rows) and inputs of any strides, sum in fp32, and round a result once.  On the GPU they run the kernels of
 ``csrc/ffn_*.hip`` on the current stream and can be captured into a graph; on the CPU the same functions are plain PyTorch.
-Arguments that do not fit raise ``ValueError``.
+Arguments that do not fit raise ``ValueError``; so do, on the GPU, more than 2^30 rows and products of more than 2^26 columns.
 """
 from __future__ import annotations
 

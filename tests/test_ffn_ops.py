@@ -174,3 +174,21 @@ def test_channel_gate_beside_a_single_row():
         assert all(torch.equal(a, b[0]) for a, b in zip(got, want))
     with pytest.raises(ValueError):                                  # vectors of two types
         ops.residual_norm(x, y, gate=g, pre_weight=w.to(dtype))
+
+
+def test_plans_fit_a_launch():
+    """A launch has fewer than 2^32 threads: the tiles of many rows are large enough for that (256 threads for 128 x 128, 512 else)."""
+    ext = ops.load_ext()
+    if ext is None:
+        pytest.skip("extension not built")
+    for name in ("fp32", "bf16", "fp16"):
+        for what, M, K, N, gated in (("forward", 2 ** 28 + 3, 8, 8, False), ("forward", 2 ** 30, 8, 5, False),
+                                     ("forward", 2 ** 28, 8, 64, True), ("dx", 2 ** 29, 64, 8, True), ("dw", 2 ** 29, 2 ** 26, 5, False)):
+            rows, cols, _ = ext.product_plan(what, name, M, K, N, gated)
+            m, n, outs = {"forward": (M, N, 1), "dx": (M, K, 1), "dw": (N, K, 1 + gated)}[what]
+            tiles = -(-m // rows) * -(-n // cols) * outs
+            assert tiles * (256 if rows == 128 and cols in (64, 128) else 512) < 2 ** 32, (name, what, M, K, N, gated)
+    with pytest.raises(ValueError):
+        ext.product_plan("forward", "fp32", 64, 2 ** 26 + 1, 64, False)
+    with pytest.raises(ValueError):
+        ext.product_plan("forward", "fp32", 2 ** 30 + 1, 64, 64, False)

@@ -4,7 +4,7 @@ in an unusual layout, the explicit forward / backward pairs, sizes at the limits
 import pytest
 import torch
 
-from test_gpu_ffn import IDS, TYPES, check_gated, check_linear, product_bounds, rnd
+from test_gpu_ffn import IDS, TYPES, check_gated, check_linear, close, product_bounds, rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -191,3 +191,47 @@ def test_channel_gate_beside_a_single_row(dev, dtype):
         a = torch.autograd.grad(one, (X, Y, g, w), (dr, dh))
         b = torch.autograd.grad(two, (X, Y, g, w), (dr[None], dh[None]))
         assert all(torch.equal(p, q[0]) for p, q in zip(one, two)) and all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+# ---- many rows -----------------------------------------------------------------------------------------------------------------
+def test_more_rows_than_one_line_of_workgroups(dev):
+    """A launch has fewer than 2^32 threads and 65536 workgroups along x here: all rows are reached, also where each has a workgroup."""
+    from ddl import ops
+    for dtype, M, C in ((torch.float16, 2 ** 26 + 5, 4), (torch.bfloat16, 70003, 4104), (torch.float32, 65537, 16384)):
+        w = rnd(dev, dtype, C, seed=2).requires_grad_(True)
+        x = torch.zeros(M, C, dtype=dtype, device=dev)
+        some = torch.tensor([0, 1, 65535, 65536, M // 2, M - 2, M - 1], device=dev)
+        x[some] = rnd(dev, dtype, 7, C, seed=1)
+        x.requires_grad_(True)
+        _, h = ops.residual_norm(x, pre_weight=w)
+        part = x.detach()[some].requires_grad_(True)
+        _, want = ops.residual_norm(part, pre_weight=w)
+        others = torch.ones(M, dtype=torch.bool, device=dev).index_fill_(0, some, False)
+        assert torch.equal(h[some], want) and not (h.any(1) & others).any()
+        dh = torch.zeros_like(h)
+        dh[some] = 1
+        (dx,) = torch.autograd.grad(h, x, dh)
+        assert torch.equal(dx[some], torch.autograd.grad(want, part, torch.ones_like(want))[0])
+        assert not (dx.any(1) & others).any()
+
+
+def test_products_of_many_rows(dev):
+    from ddl import ops
+    M = 2 ** 28 + 3
+    x, w = torch.zeros(M, 8, dtype=torch.bfloat16, device=dev), rnd(dev, torch.bfloat16, 8, 8, seed=1)
+    some = torch.tensor([0, 1, 2 ** 27, M - 2, M - 1], device=dev)
+    x[some] = rnd(dev, torch.bfloat16, 5, 8, seed=2)
+    y = ops.linear(x, w)
+    want, bound = product_bounds(x[some].double(), w.double(), None, "none")
+    close(y[some], want, bound, torch.bfloat16, "y")
+    assert (y[2:2 ** 27] == 0).all()
+
+
+def test_widths_beyond_the_limit_are_refused(dev):
+    """Nothing is allocated: the weights have no columns, or no rows."""
+    from ddl import ops
+    wide = 2 ** 26 + 1
+    with pytest.raises(ValueError, match="columns"):
+        ops.linear(torch.empty(1, 0, device=dev), torch.empty(wide, 0, device=dev))
+    with pytest.raises(ValueError, match="columns"):
+        ops.gated_linear(torch.empty(0, wide, device=dev), torch.empty(0, wide, device=dev), torch.empty(0, wide, device=dev))

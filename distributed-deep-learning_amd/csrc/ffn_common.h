@@ -52,7 +52,9 @@ __device__ __forceinline__ float act_grad(int act, float z, float& a) {
     case ACT_GELU_TANH: {
       const float s = sigmoid_f(gelu_tanh_arg(z));
       a = z * s;
-      return s + z * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * z * z);
+      // beyond 12 s is 0 or 1, and the second term nothing: from 2e19 on its square would be infinite (a NaN stays one)
+      const float c = z > 12.f ? 12.f : z < -12.f ? -12.f : z;
+      return s + c * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * c * c);
     }
     case ACT_SIGMOID: a = sigmoid_f(z); return a * (1.0f - a);
     default: a = z; return 1.f;

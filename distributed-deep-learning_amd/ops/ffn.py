@@ -55,7 +55,8 @@ def _act(z: torch.Tensor, activation: str) -> torch.Tensor:
     if activation == "gelu":
         return 0.5 * z * (1 + torch.erf(z * math.sqrt(0.5)))
     if activation == "gelu_tanh":
-        return z * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))
+        c = z.clamp(-12, 12)                     # beyond, the sigmoid is 0 or 1 in fp32, and the cube would overflow in its derivative
+        return z * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (c + 0.044715 * c ** 3))
     return torch.sigmoid(z) if activation == "sigmoid" else z
 
 

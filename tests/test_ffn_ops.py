@@ -192,3 +192,30 @@ def test_plans_fit_a_launch():
         ext.product_plan("forward", "fp32", 64, 2 ** 26 + 1, 64, False)
     with pytest.raises(ValueError):
         ext.product_plan("forward", "fp32", 2 ** 30 + 1, 64, 64, False)
+
+
+FAR = (1e4, 1e12, 1e20, 1e30)
+
+
+def check_far_sums(device):
+    """Activations and slopes of sums far from zero are their limits, with no infinity or NaN on the way."""
+    for act in ops.ACTIVATIONS:
+        for z in FAR:
+            for sign in (1.0, -1.0):
+                x = torch.full((3, 1), sign * z ** 0.5, device=device, requires_grad=True)
+                w = torch.full((1, 1), z ** 0.5, device=device, requires_grad=True)
+                value = {"none": sign * z, "sigmoid": max(sign, 0.0)}.get(act, max(sign, 0.0) * z)
+                slope = {"none": 1.0, "sigmoid": 0.0}.get(act, max(sign, 0.0))
+                y = ops.linear(x, w, activation=act)
+                dx, dw = torch.autograd.grad(y.sum(), (x, w))
+                for got, want in ((y, value), (dx, slope * z ** 0.5), (dw, 3 * slope * sign * z ** 0.5)):
+                    torch.testing.assert_close(got, torch.full_like(got, want), rtol=1e-5, atol=1e-30)
+                up = (w.detach() / z).requires_grad_(True)             # x times this: the sign
+                h = ops.gated_linear(x, w, up, activation=act)
+                torch.testing.assert_close(h, torch.full_like(h, value * sign), rtol=1e-5, atol=1e-30)
+                (dw,) = torch.autograd.grad(h.sum(), w)
+                torch.testing.assert_close(dw, torch.full_like(dw, 3 * slope * z ** 0.5), rtol=1e-5, atol=1e-30)
+
+
+def test_far_sums():
+    check_far_sums("cpu")

@@ -235,3 +235,8 @@ def test_widths_beyond_the_limit_are_refused(dev):
         ops.linear(torch.empty(1, 0, device=dev), torch.empty(wide, 0, device=dev))
     with pytest.raises(ValueError, match="columns"):
         ops.gated_linear(torch.empty(0, wide, device=dev), torch.empty(0, wide, device=dev), torch.empty(0, wide, device=dev))
+
+
+def test_far_sums(dev):
+    from test_ffn_ops import check_far_sums
+    check_far_sums(dev)

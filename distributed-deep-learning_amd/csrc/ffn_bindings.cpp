@@ -571,7 +571,7 @@ void check_dropout(const Tensor& x, double p, const Tensor& key, const OptT& res
   BAD_UNLESS(x.is_cuda(), "dropout: GPU tensor expected");
   type_of(x, "dropout");
   BAD_UNLESS(p >= 0. && p <= 1., "dropout: p must lie in [0, 1], got ", p);
-  BAD_UNLESS(key.scalar_type() == at::kLong && key.numel() == 2 && key.is_contiguous() && key.device() == x.device(),
+  BAD_UNLESS(key.scalar_type() == at::kLong && key.numel() == 2 && key.device() == x.device(),
              "dropout: key must be two int64 values (seed, call) on the input's device");
   if (has(res)) {
     check_like(*res, x, "dropout", "residual");
@@ -581,14 +581,14 @@ void check_dropout(const Tensor& x, double p, const Tensor& key, const OptT& res
 Tensor dropout_apply(const Tensor& x, double p, const Tensor& key, const OptT& res) {
   check_dropout(x, p, key, res);
   ddl::DeviceGuard guard(x.device());
-  const Tensor xc = x.contiguous(), rc = has(res) ? res->contiguous() : Tensor();
+  const Tensor xc = x.contiguous(), rc = has(res) ? res->contiguous() : Tensor(), kc = key.contiguous();
   Tensor y = at::empty(x.sizes(), x.options());
   ffn::DropoutArgs a;
   a.x = xc.data_ptr();
   a.residual = rc.defined() ? rc.data_ptr() : nullptr;
   a.y = y.data_ptr();
   a.n = x.numel();
-  a.key = key.data_ptr<int64_t>();
+  a.key = kc.data_ptr<int64_t>();
   a.p = p;
   ffn::launch_dropout(type_of(x, "dropout"), a, cur_stream());
   return y;

@@ -240,3 +240,19 @@ def test_widths_beyond_the_limit_are_refused(dev):
 def test_far_sums(dev):
     from test_ffn_ops import check_far_sums
     check_far_sums(dev)
+
+
+def test_a_key_in_any_layout(dev):
+    """Two int64 values, as on the CPU: a column of a table, a [2, 1] tensor, one value for both."""
+    from ddl import ops
+    x, k = rnd(dev, torch.float32, 40, 30), torch.tensor([7, 9], device=dev)
+    want = ops.dropout(x, 0.5, k)
+    table = torch.stack([k, k + 1], 1)
+    for key in (table[:, 0], k.view(2, 1), table[:, :1]):
+        leaf = x.clone().requires_grad_(True)
+        y = ops.dropout(leaf, 0.5, key)
+        assert torch.equal(y, want)
+        (dx,) = torch.autograd.grad(y, leaf, x)
+        assert torch.equal(dx, want)
+    same = torch.tensor(7, device=dev).expand(2)
+    assert torch.equal(ops.dropout(x, 0.5, same), ops.dropout(x, 0.5, same.contiguous()))

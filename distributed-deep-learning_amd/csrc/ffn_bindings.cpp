@@ -869,12 +869,13 @@ void register_ffn_ops(pybind11::module_& m) {
   m.def("rng_keys", &rng_keys, "state (seed, calls) -> n keys (seed, call); calls += n");
   m.def("residual_norm", &residual_norm);
   m.def("norm_forward", [](const Tensor& x, const OptT& y, const OptT& gate, const OptT& post_w, const OptT& post_b, const OptT& pre_w,
-                           const OptT& pre_b, bool layer, double eps, double scale) {
+                           const OptT& pre_b, bool layer, double eps, double scale, bool keep) {
     const NormIn in = norm_in(x, y, gate, post_w, post_b, pre_w, pre_b, layer, eps, scale);
     check_norm(in);
     ddl::DeviceGuard guard(x.device());
-    return norm_forward(contiguous(in), true);
-  }, "-> (r, h, statistics)");
+    return norm_forward(contiguous(in), keep);
+  }, "-> (r, h, statistics)", py::arg("x"), py::arg("branch"), py::arg("gate"), py::arg("post_weight"), py::arg("post_bias"),
+        py::arg("pre_weight"), py::arg("pre_bias"), py::arg("layer"), py::arg("eps"), py::arg("scale"), py::arg("keep") = true);
   m.def("norm_backward", [](const Tensor& x, const OptT& y, const OptT& gate, const OptT& post_w, const OptT& post_b, const OptT& pre_w,
                             const OptT& pre_b, bool layer, double eps, double scale, const Tensor& stats, const OptT& dr, const OptT& dh) {
     const NormIn in = norm_in(x, y, gate, post_w, post_b, pre_w, pre_b, layer, eps, scale);

@@ -80,16 +80,18 @@ PARAMS = ("norm_in.weight", "norm_in.bias", "gate.weight", "up.weight", "gate.bi
 LAYER_NORM_EPS = 1e-5
 
 
-def native_forward(ext, p: Dict[str, torch.Tensor], f: torch.Tensor, drop: float,
-                   key: Optional[torch.Tensor]) -> Tuple[torch.Tensor, Tuple[torch.Tensor, ...]]:
-    """The block on the parameter views of the native engine: (h, what the backward pass needs).  ``key`` None: no dropout."""
+def native_forward(ext, p: Dict[str, torch.Tensor], f: torch.Tensor, drop: float, key: Optional[torch.Tensor],
+                   keep: bool) -> Tuple[torch.Tensor, Tuple[Optional[torch.Tensor], ...]]:
+    """The block on the parameter views of the native engine: (h, what the backward pass needs).  ``key`` None: no dropout.  ``keep``:
+    a backward pass may follow; otherwise neither the projections' sums nor the norms' statistics are written."""
     silu = ops.ACTIVATIONS.index("silu")
-    _, n, s_in = ext.norm_forward(f, None, None, None, None, p["norm_in.weight"], p["norm_in.bias"], True, LAYER_NORM_EPS, 1.0)
-    g, z = ext.gated_forward(n, p["gate.weight"], p["up.weight"], p["gate.bias"], p["up.bias"], silu, True)
+    _, n, s_in = ext.norm_forward(f, None, None, None, None, p["norm_in.weight"], p["norm_in.bias"], True, LAYER_NORM_EPS, 1.0, keep)
+    g, z = ext.gated_forward(n, p["gate.weight"], p["up.weight"], p["gate.bias"], p["up.bias"], silu, keep)
     y, _ = ext.linear_forward(g, p["down.weight"], p["down.bias"], None, 0, False)
     if key is not None:
         y = ext.dropout(y, drop, key, None)
-    _, h, s_out = ext.norm_forward(f, y, p["scale"], None, None, p["norm_out.weight"], p["norm_out.bias"], True, LAYER_NORM_EPS, 1.0)
+    _, h, s_out = ext.norm_forward(f, y, p["scale"], None, None, p["norm_out.weight"], p["norm_out.bias"], True, LAYER_NORM_EPS, 1.0,
+                                   keep)
     return h, (f, n, s_in, z, g, y, s_out)
 
 

@@ -486,7 +486,7 @@ class TransitionUnit:
 # ======================================================================================
 class _HeadFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, buf: torch.Tensor, anchor: torch.Tensor, unit: "HeadUnit", in_stats):
+    def forward(ctx, buf: torch.Tensor, anchor: torch.Tensor, unit: "HeadUnit", in_stats, keep: bool):
         ext = _ext()
         train = unit.stage.training
         B, H, W, C = buf.shape
@@ -509,7 +509,7 @@ class _HeadFn(torch.autograd.Function):
         ffn = ()
         if unit.ffn is not None:             # residual feed-forward block in front of the classifier (models/head.py)
             key = unit.stage.dropout_key() if train and unit.drop > 0 else None
-            pooled, ffn = gated_head.native_forward(ext, unit.ffn, pooled, unit.drop, key)
+            pooled, ffn = gated_head.native_forward(ext, unit.ffn, pooled, unit.drop, key, keep)
             ffn += () if key is None else (key,)
         logits = ext.linear_fwd(pooled, unit.cw, unit.cb)
         ctx.unit = unit
@@ -541,7 +541,7 @@ class _HeadFn(torch.autograd.Function):
             ext.rows_op(4, M, d2d, buf2d, k[1], k[2], d2d, H, W, False)
         unit.stage._unit_grads_ready(unit)
         unit.stage._owned_grad_ptr = dbuf.data_ptr()
-        return dbuf, None, None, None
+        return dbuf, None, None, None, None
 
 
 class HeadUnit:
@@ -567,7 +567,7 @@ class HeadUnit:
             self.param_names += ["ffn." + n for n in gated_head.PARAMS]
 
     def __call__(self, x, in_stats):
-        return _HeadFn.apply(x, self.stage.anchor, self, in_stats), None
+        return _HeadFn.apply(x, self.stage.anchor, self, in_stats, torch.is_grad_enabled()), None
 
 
 # ======================================================================================

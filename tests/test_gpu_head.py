@@ -126,3 +126,29 @@ def test_pipeline_lanes_draw_the_serial_masks(dev, fwd_lanes):
         torch.cuda.synchronize()
         finals.append((losses, strat.arena.flat_param.clone()))
     assert finals[0][0] == finals[1][0] and torch.equal(finals[0][1], finals[1][1])
+
+
+def test_evaluation_keeps_nothing_for_a_backward_pass(dev):
+    """Without gradients neither the projections' fp32 sums nor the norms' statistics are written; the logits are the same."""
+    from ddl.models import head
+    native, _ = _stages(dev, 0.2)
+    native.eval()
+    B, width, made = 40, 200, {}
+    x = torch.randn(B, 7, 7, 1024, generator=torch.Generator().manual_seed(1)).to(dev)
+
+    def run(grad):
+        with torch.set_grad_enabled(grad):
+            before = torch.cuda.memory_stats()["allocated_bytes.all.allocated"]
+            y = native(x)
+            return y.detach(), torch.cuda.memory_stats()["allocated_bytes.all.allocated"] - before
+
+    run(False)
+    (a, plain), (b, kept) = run(False), run(True)
+    assert torch.equal(a, b)
+    assert kept - plain >= 2 * B * width * 4 + 2 * 4 * B * 4          # two planes of sums, the statistics of two norms
+    ext = head.ops.require_ext()
+    unit = native.unit_objs[-1]
+    f = torch.randn(B, 1024, generator=torch.Generator().manual_seed(2)).to(dev)
+    h, saved = head.native_forward(ext, unit.ffn, f, 0.0, None, False)
+    again, _ = head.native_forward(ext, unit.ffn, f, 0.0, None, True)
+    assert torch.equal(h, again) and [t is None for t in saved] == [False, False, True, True, False, False, True]

@@ -60,8 +60,11 @@ class GatedHead(nn.Module):
         self._rng: Optional[ops.DropoutRng] = None
 
     def rng(self, device) -> ops.DropoutRng:
+        """The keys' generator on ``device``; it goes where the features go, and on with its sequence."""
         if self._rng is None:
             self._rng = ops.DropoutRng(dropout_seed(), device)
+        elif self._rng.state.device != torch.device(device):
+            self._rng.state = self._rng.state.to(device)
         return self._rng
 
     def forward(self, f: torch.Tensor) -> torch.Tensor:

@@ -152,3 +152,19 @@ def test_evaluation_keeps_nothing_for_a_backward_pass(dev):
     h, saved = head.native_forward(ext, unit.ffn, f, 0.0, None, False)
     again, _ = head.native_forward(ext, unit.ffn, f, 0.0, None, True)
     assert torch.equal(h, again) and [t is None for t in saved] == [False, False, True, True, False, False, True]
+
+
+def test_portable_head_moves_between_devices(dev):
+    """A step on the CPU, then .to(GPU): the next step draws the next mask there."""
+    from ddl.models import HeadConfig
+    from ddl.models.head import GatedHead
+    torch.manual_seed(4)
+    m = GatedHead(40, HeadConfig("gated", width=48, dropout=0.25))
+    f = torch.randn(6, 40)
+    m(f)
+    state = m.rng("cpu").state.tolist()
+    m.to(dev)
+    got = m(f.to(dev))
+    keep = torch.from_numpy(oracle.kept(state, 240, 0.25)).double().view(6, 40) / 0.75
+    assert (got.cpu().double() - block64(m.cpu(), f.double(), keep)).abs().max() < 1.6e-4       # the bound of tests/test_head.py
+    assert m.rng(dev).state.tolist() == [state[0], state[1] + 1]

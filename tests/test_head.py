@@ -71,3 +71,13 @@ def test_entry_scripts_train_with_the_gated_head(tmp_path):
                 "--snapshot-epoch", "0", *head], env)
     assert "Resuming training from snapshot at Epoch 1" in out
     _torchrun(2, "pp.py", [*SMALL, "--batch-size", "10", *head], env)
+
+
+def test_dropout_keys_move_with_the_head():
+    m = GatedHead(40, CFG)
+    m.train()
+    m(torch.randn(6, 40))
+    key = m.rng("cpu").state.tolist()
+    assert m.rng(torch.device("meta")).state.device.type == "meta"
+    m._rng.state = torch.tensor(key)
+    assert m.rng("cpu").state.tolist() == key and key[1] == 1

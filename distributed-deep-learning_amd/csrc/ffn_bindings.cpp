@@ -302,11 +302,15 @@ ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width,
   // rounding that makes a gradient's error sqrt(2) times one rounding, where many of them average.  Few rows may not average (one
   // row, 64 columns: 1.57 times the rounding alone, four columns: 3), and their products have time to spare.  So up to FEW_ROWS rows
   // dz comes in two parts, the rounded one in rows 0 .. M-1 and what it lacks in rows M .. 2M-1: d_x sums both rows' outputs in
-  // fp32 before it rounds, d_w adds the parts before it multiplies.
+  // fp32 before it rounds, d_w adds the parts before it multiplies.  Above that the other way, two parts for every product, was not taken:
+  // the matrix cores are what bounds the large ones, and both gradients would multiply twice as much.
+  // fp16: dz, which is no result, may lie outside the type's range where the gradients lie inside.  It is held times a power of two
+  // (act_bwd_rescale_kernel), and the products' fp32 sums are scaled back.
   const bool make_dz = z.defined() && (need_dx || need_dw);
   const bool few = M <= ffn::FEW_ROWS, two = make_dz && dtype != ffn::F32 && few;
   const int R = two ? 2 * M : M;
-  Tensor dz;
+  Tensor dz, range;
+  const float* scale = nullptr;                                      // what dz is held in (fp16)
   Operand dzo[2], wo[2], xo;
   ffn::PackArgs todo;
   if (make_dz) {
@@ -339,6 +343,12 @@ ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width,
         if (make_dz) b.dz[d] = const_cast<void*>(dzo[d].p);
       }
     b.chunks = ffn::act_bwd_chunks(dtype, M, N);
+    if (make_dz && dtype == ffn::F16) {
+      const int64_t tiles = ffn::act_bwd_tiles(dtype, b);
+      range = at::empty({tiles + 1}, x.options().dtype(at::kFloat));
+      b.range = range.data_ptr<float>();
+      scale = b.scale = b.range + tiles;
+    }
     void* outs[2] = {need_db ? r.db[0].data_ptr() : nullptr, need_db && dual ? r.db[1].data_ptr() : nullptr};
     if (need_db && b.chunks == 1) {
       b.db[0] = outs[0];
@@ -361,6 +371,7 @@ ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width,
       g.q[d] = dzo[d].p; g.ldq[d] = dzo[d].ld;
     }
     set_out(g.ep, 0, r.dx);
+    g.ep.scale = scale;
     run_gemm(dtype, g, x);
   }
   if (need_dw && few) {
@@ -371,6 +382,7 @@ ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width,
     o.ldx = row_stride(x2);
     o.x_vec = rows_aligned(x2);
     o.two = two;
+    o.scale = scale;
     o.ldd = make_dz ? dzo[0].ld : row_stride(dy2);
     o.out_vec = (int64_t)K * x.element_size() % 16 == 0;
     for (int d = 0; d < D; ++d) {
@@ -385,6 +397,7 @@ ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width,
       g.q[d] = dzo[d].p; g.ldq[d] = dzo[d].ld;
       set_out(g.ep, d, r.dw[d]);
     }
+    g.ep.scale = scale;
     run_gemm(dtype, g, x);
   }
   return r;

@@ -105,6 +105,7 @@ struct Epilogue {
   long ldz = 0;
   int act = ACT_NONE;
   bool out_vec = false, res_vec = false, bias_vec = false;   // rows start 16-byte aligned
+  const float* scale = nullptr;           // fp16 gradients: the power of two that dz is held in (device; see act_bwd_rescale_kernel)
 };
 
 // act over V values; one switch for all of them
@@ -218,6 +219,8 @@ struct ActBwdArgs {
   void* dz[2] = {nullptr, nullptr};       // padded rows; may be null where only the column sums are wanted
   long ldd = 0;
   bool two = false;                       // dz in two parts: rounded, and what that lacks in rows M ..
+  float* range = nullptr;                 // fp16 with dz: [act_bwd_tiles] largest finite |dz| of each workgroup
+  float* scale = nullptr;                 // fp16 with dz: the power of two that dz is held in
   int act = ACT_NONE;
   bool dual = false;
   int M = 0, N = 0;
@@ -234,9 +237,11 @@ struct OuterArgs {
   int M = 0, N = 0, K = 0, nout = 1;
   int rows = 0, strips = 0;               // of the output: rows a workgroup writes, strips of 1024 columns (the launcher's)
   bool two = false, x_vec = false, out_vec = false;
+  const float* scale = nullptr;           // of dz (fp16), null: 1
 };
 void launch_outer(int dtype, const OuterArgs& a, hipStream_t s);
 int act_bwd_chunks(int dtype, int M, int N);
+int act_bwd_tiles(int dtype, const ActBwdArgs& a);         // workgroups of the launch
 void launch_act_bwd(int dtype, const ActBwdArgs& a, hipStream_t s);
 // out[which][n] = sum over chunks of part[chunk][which][n]
 void launch_colsum(int out_dtype, const float* part, int chunks, int nvec, long n, void* const* out, hipStream_t s);

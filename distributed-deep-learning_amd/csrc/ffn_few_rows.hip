@@ -114,12 +114,14 @@ __global__ void __launch_bounds__(256) outer_kernel(OuterArgs a) {
   const long n0 = (long)(blockIdx.x / a.strips) * a.rows;
   const int count = (int)min((long)a.rows, a.N - n0);
   const T* src = (const T*)a.dz[which] + n0;
+  const float scale = a.scale != nullptr ? *a.scale : 1.f;
   for (int i = threadIdx.x; i < a.rows * MR; i += 256) {
     const int n = i % a.rows, m = i / a.rows;
     float v = 0.f;
     if (m < a.M && n < count) {
       v = to_f(src[m * a.ldd + n]);
       if (a.two) v += to_f(src[(m + a.M) * a.ldd + n]);
+      v *= scale;
     }
     dz[n][m] = v;
   }

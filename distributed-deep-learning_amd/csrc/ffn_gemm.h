@@ -213,6 +213,9 @@ __device__ __forceinline__ void finish(const GemmArgs& a, const f32x4 (&acc)[NT]
     }
   }
   constexpr bool Z_ROWS = DUAL && CHUNK > 0;               // z is written by itself below
+  constexpr bool SCALED = PLAIN && std::is_same<T, _Float16>::value;
+  float scale = 1.f;
+  if (SCALED && a.partial == nullptr && a.ep.scale != nullptr) scale = *a.ep.scale;
   // the sums of row m
   auto row = [&](int m, const f32x4 (&sums)[NT]) {
     if (m >= a.M) return;
@@ -223,6 +226,7 @@ __device__ __forceinline__ void finish(const GemmArgs& a, const f32x4 (&acc)[NT]
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         v[e] = sums[p * TPV + e / 4][e % 4];
+        if (SCALED) v[e] *= scale;
         w[e] = DUAL ? sums[(DUAL ? NT / 2 : 0) + p * TPV + e / 4][e % 4] : 0.f;
       }
       if (a.partial != nullptr) {                          // rows of whole vectors: ldw is N rounded up to 16

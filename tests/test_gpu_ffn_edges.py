@@ -4,7 +4,8 @@ in an unusual layout, the explicit forward / backward pairs, sizes at the limits
 import pytest
 import torch
 
-from test_gpu_ffn import IDS, TYPES, check_gated, check_linear, close, product_bounds, rnd
+import ffn_oracle as oracle
+from test_gpu_ffn import EPS, IDS, TYPES, act_and_slope, check_gated, check_linear, close, product_bounds, rnd, slope_bound, tiny
 
 pytestmark = pytest.mark.gpu
 
@@ -256,3 +257,114 @@ def test_a_key_in_any_layout(dev):
         assert torch.equal(dx, want)
     same = torch.tensor(7, device=dev).expand(2)
     assert torch.equal(ops.dropout(x, 0.5, same), ops.dropout(x, 0.5, same.contiguous()))
+
+
+# ---- fp16: dz outside the type's range, gradients inside ----------------------------------------------------------------------
+def gradient_bounds(x, w, b, act, dy, dtype):
+    """(dz of each weight, its bound) in 64 bits.  dz is held rounded to `dtype` times a power of two 2^e: off by half a step, u of itself,
+    or 2^-25 2^e in fp16 where it is small; 2^e is at most 2^-14 of the largest unless that lies in [2^-8, 65504], where it is 1."""
+    X, W, B, D = x.double(), [t.double() for t in w], None if b is None else b.double(), dy.double()
+    z, zerr = product_bounds(X, W[0], B, act)
+    a, da = act_and_slope(z, act)
+    serr = slope_bound(z, zerr, act)
+    if len(w) == 2:
+        up, uerr = product_bounds(X, W[1], B, act)
+        aerr = 1.13 * zerr + 16 * EPS * (a.abs() + z.abs())
+        dz = [D * up * da, D * a]
+        e32 = [D.abs() * (serr * (up.abs() + uerr) + da.abs() * uerr) + 8 * EPS * dz[0].abs(), D.abs() * aerr + 8 * EPS * dz[1].abs()]
+    else:
+        dz = [D * da]
+        e32 = [D.abs() * serr + 4 * EPS * dz[0].abs()]
+    top, u = max(d.abs().max().item() for d in dz), oracle.rounding(dtype)
+    step = tiny(dtype) if 2.0 ** -8 <= top <= 65504 else 2.0 ** -39 * top
+    return dz, [e + u * (d.abs() + e) + step for d, e in zip(dz, e32)], top
+
+
+def check_gradients(ops, x, w, b, act, dy, dtype, got):
+    dz, err, top = gradient_bounds(x, w, b, act, dy, dtype)
+    M, N = dy.shape
+    X, W = x.double(), [t.double() for t in w]
+    size = sum(d.abs() @ v.abs() for d, v in zip(dz, W))
+    want = [sum(d @ v for d, v in zip(dz, W))] + [d.T @ X for d in dz]
+    bound = [sum(e @ v.abs() for e, v in zip(err, W)) + (2 * N + 16) * EPS * size]
+    bound += [e.T @ X.abs() + (M + 16) * EPS * (d.abs().T @ X.abs()) for d, e in zip(dz, err)]
+    for t, v, e, what in zip(got, want, bound, ("dx", "dw 0", "dw 1")):
+        assert v.abs().max() + e.max() < 65504, f"{what} itself is out of range"
+        close(t, v, e, dtype, what)
+    return top
+
+
+#: scales of x, w_gate (or w), w_up, dy; the range of the largest |dz|
+RANGES = {"beyond": ((0.01, 1e-3, 1e4, 300.0), (65504, 1e9)), "below": ((100.0, 1e-3, 1e-3, 2e-6), (1e-9, 2.0 ** -13)),
+          "inside": ((1.0, 0.1, 0.1, 1.0), (2.0 ** -8, 65504))}
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("where", list(RANGES))
+@pytest.mark.parametrize("M", [1, 5, 32, 33, 300, 2500])
+def test_gradients_of_dz_out_of_range(dev, dtype, where, M):
+    from ddl import ops
+    K, N = (64, 72) if M < 2500 else (1024, 2052)
+    (sx, sg, su, sd), (lo, hi) = RANGES[where]
+    if where == "beyond" and M > 32:
+        sx *= (32 / M) ** 0.5                                          # d_w, a sum over M rows, has to stay in range itself
+    fan = (64 / K) ** 0.5                                              # the sums of the small case, also at K = 1024
+    x, dy = rnd(dev, dtype, M, K, seed=1, scale=sx), rnd(dev, dtype, M, N, seed=2, scale=sd)
+    g, u = rnd(dev, dtype, N, K, seed=3, scale=sg * fan), rnd(dev, dtype, N, K, seed=4, scale=su * fan)
+    leaves = [t.requires_grad_(True) for t in (x, g, u)]
+    got = torch.autograd.grad(ops.gated_linear(*leaves), leaves, dy)
+    top = check_gradients(ops, x.detach(), [g.detach(), u.detach()], None, "silu", dy, dtype, got)
+    assert M == 1 or lo <= top <= hi
+    # one weight: only the slope, up to 1.1, stands between dy and dz
+    b = torch.full((N,), 2.4, device=dev, dtype=dtype)
+    dy = (rnd(dev, torch.float32, M, N, seed=5).sign() * {"beyond": 65000.0, "below": 2e-6, "inside": 1.0}[where]).to(dtype)
+    v = (g.detach() * (1e-3 if where == "beyond" else 1.0)).to(dtype).requires_grad_(True)
+    xs = (x.detach() * (0.1 if where == "beyond" else 1.0)).to(dtype).requires_grad_(True)
+    got = torch.autograd.grad(ops.linear(xs, v, b, activation="silu"), (xs, v), dy)
+    check_gradients(ops, xs.detach(), [v.detach()], b, "silu", dy, dtype, got)
+
+
+@pytest.mark.parametrize("M", [8, 90])
+def test_captured_gradients_follow_the_range(dev, M):
+    """The power of two is chosen on the device: replays of one graph see ordinary, huge and tiny gradients in turn."""
+    from ddl import ops
+    x, g, u = (rnd(dev, torch.float16, *s, seed=i, scale=c).requires_grad_(True)
+               for i, (s, c) in enumerate((((M, 64), 0.01), ((72, 64), 1e-3), ((72, 64), 1e4))))
+    dy = torch.empty(M, 72, dtype=torch.float16, device=dev)
+
+    def step():
+        return torch.autograd.grad(ops.gated_linear(x, g, u), (x, g, u), dy)
+
+    dy.fill_(1)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i, scale in enumerate((1.0, 300.0, 1e-6, 300.0, 1.0)):
+        dy.copy_(rnd(dev, torch.float16, M, 72, seed=20 + i, scale=scale))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want))
+        check_gradients(ops, x.detach(), [g.detach(), u.detach()], None, "silu", dy, torch.float16, out)
+
+
+def test_infinite_gradients_stay_infinite(dev):
+    """An infinity or NaN in dy stays where the formula has it, whatever the scale the others are held in."""
+    from ddl import ops
+    for M in (6, 60):
+        for scale in (1.0, 3e4):
+            x, w = (rnd(dev, torch.float16, *s, seed=i, scale=0.01).requires_grad_(True) for i, s in enumerate(((M, 64), (72, 64))))
+            b = torch.full((72,), 2.4, device=dev, dtype=torch.float16)
+            dy = rnd(dev, torch.float16, M, 72, seed=3).sign() * scale
+            y = ops.linear(x, w, b, activation="silu")
+            want = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+            dy[2, 5], dy[3, 7] = float("inf"), float("nan")
+            dx, dw = torch.autograd.grad(y, (x, w), dy)
+            rows, cols = ([i for i in range(n) if i not in bad] for n, bad in ((M, (2, 3)), (72, (5, 7))))
+            assert torch.equal(dx[rows], want[0][rows]) and torch.equal(dw[cols], want[1][cols])
+            assert dx[2].isinf().all() and dx[3].isnan().all() and dw[5].isinf().all() and dw[7].isnan().all()

@@ -31,6 +31,12 @@ int type_of(const Tensor& t, const char* op) {
   BAD_UNLESS(false, op, ": float32, bfloat16 or float16 expected, got ", t.scalar_type());
   return 0;
 }
+// The tensor whose memory holds its values: PyTorch marks lazily negated views (the imaginary part of a conjugate) and zeros without
+// memory, which its own operators resolve in its dispatcher and a kernel that reads memory would not see.
+Tensor in_memory(const Tensor& t) {
+  if (!t.defined() || !(t.is_neg() || t._is_zerotensor())) return t;
+  return t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t.resolve_neg();
+}
 bool has(const OptT& t) { return t.has_value() && t->defined(); }
 Tensor get(const OptT& t) { return has(t) ? *t : Tensor(); }
 const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -208,8 +214,10 @@ std::tuple<int, int, int> product_plan(const std::string& what, const std::strin
 struct Kept { Tensor z, x, w[2]; };
 
 // One or two weights -> out [M, N].
-Tensor product_forward(const Tensor& x, const Tensor& w0, const Tensor& w1, const Tensor& b0, const Tensor& b1, const Tensor& res,
-                       int act, bool keep_sums, Kept* kept, const char* op) {
+Tensor product_forward(const Tensor& x_in, const Tensor& w0_in, const Tensor& w1_in, const Tensor& b0_in, const Tensor& b1_in,
+                       const Tensor& res_in, int act, bool keep_sums, Kept* kept, const char* op) {
+  const Tensor x = in_memory(x_in), w0 = in_memory(w0_in), w1 = in_memory(w1_in), b0 = in_memory(b0_in), b1 = in_memory(b1_in),
+               res = in_memory(res_in);
   const int dtype = type_of(x, op);
   const Tensor x2 = rows_of(x);
   const int M = rows_fit(x2.size(0), op), K = width_fits(x2.size(1), op), N = width_fits(w0.size(0), op);
@@ -278,9 +286,9 @@ struct ProductGrads { Tensor dx, dw[2], db[2]; };
 ProductGrads product_backward(const Tensor& dy, const Kept& kept, int64_t width, int act, bool need_dx, bool need_dw, bool need_db,
                               const char* op) {
   not_recorded(op);
-  const Tensor &x = kept.x, &w0 = kept.w[0], &w1 = kept.w[1], &z = kept.z;
+  const Tensor x = in_memory(kept.x), w0 = in_memory(kept.w[0]), w1 = in_memory(kept.w[1]), &z = kept.z;
   const int dtype = type_of(x, op);
-  const Tensor x2 = rows_of(x), dy2 = rows_of(dy);
+  const Tensor x2 = rows_of(x), dy2 = rows_of(in_memory(dy));
   const int M = rows_fit(dy2.size(0), op), K = width_fits(width, op), N = width_fits(dy2.size(1), op);
   const bool dual = w1.defined();
   const int D = dual ? 2 : 1;
@@ -594,7 +602,8 @@ void check_dropout(const Tensor& x, double p, const Tensor& key, const OptT& res
 Tensor dropout_apply(const Tensor& x, double p, const Tensor& key, const OptT& res) {
   check_dropout(x, p, key, res);
   ddl::DeviceGuard guard(x.device());
-  const Tensor xc = x.contiguous(), rc = has(res) ? res->contiguous() : Tensor(), kc = key.contiguous();
+  const Tensor xc = in_memory(x).contiguous(), rc = has(res) ? in_memory(*res).contiguous() : Tensor(),
+               kc = in_memory(key).contiguous();
   Tensor y = at::empty(x.sizes(), x.options());
   ffn::DropoutArgs a;
   a.x = xc.data_ptr();
@@ -704,7 +713,7 @@ void check_norm(const NormIn& in) {
 NormIn contiguous(const NormIn& in) {
   NormIn c = in;
   for (Tensor* t : {&c.x, &c.y, &c.gate, &c.post_w, &c.post_b, &c.pre_w, &c.pre_b})
-    if (t->defined()) *t = t->contiguous();
+    if (t->defined()) *t = in_memory(*t).contiguous();
   return c;
 }
 // of checked, contiguous inputs
@@ -760,7 +769,7 @@ NormGrads norm_backward(const NormIn& in, const Tensor& st, const Tensor& dr, co
     no_tangent(t, "residual_norm");
     check_like(t, in.x, "residual_norm", "an output's gradient");
     BAD_UNLESS(t.sizes() == in.x.sizes(), "residual_norm: gradient ", t.sizes(), " where x is ", in.x.sizes());
-    c = t.contiguous();
+    c = in_memory(t).contiguous();
     a.vec = a.vec && aligned(c.data_ptr());
     return c.data_ptr();
   };

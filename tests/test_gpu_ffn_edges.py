@@ -368,3 +368,35 @@ def test_infinite_gradients_stay_infinite(dev):
             rows, cols = ([i for i in range(n) if i not in bad] for n, bad in ((M, (2, 3)), (72, (5, 7))))
             assert torch.equal(dx[rows], want[0][rows]) and torch.equal(dw[cols], want[1][cols])
             assert dx[2].isinf().all() and dx[3].isnan().all() and dw[5].isinf().all() and dw[7].isnan().all()
+
+
+# ---- tensors whose memory does not hold their values -----------------------------------------------------------------------------
+def test_negated_views(dev):
+    """The imaginary part of a conjugate is a lazily negated view: every operator sees its values, in every place, gradients as well."""
+    from ddl import ops
+
+    def negated(t):
+        v = torch.complex(torch.zeros_like(t), -t).conj().imag
+        assert v.is_neg() and torch.equal(v, t)
+        return v
+
+    key = torch.tensor([1, 2], device=dev)
+    for M in (5, 50):
+        x, y, res = (rnd(dev, torch.float32, M, 24, seed=i) for i in range(3))
+        w, v = rnd(dev, torch.float32, 24, 24, seed=4), rnd(dev, torch.float32, 24, seed=5)
+        calls = [lambda x, y, res, w, v: [ops.linear(x, w, v, activation="silu", residual=res)],
+                 lambda x, y, res, w, v: [ops.gated_linear(x, w, w, v, v)],
+                 lambda x, y, res, w, v: [ops.dropout(x, 0.3, key, residual=res)],
+                 lambda x, y, res, w, v: ops.residual_norm(x, y, kind="layer", pre_weight=v, pre_bias=v, post_weight=v, post_bias=v, gate=v),
+                 lambda x, y, res, w, v: ops.residual_norm(x, y, gate=res, pre_weight=v)]
+        for i, call in enumerate(calls):
+            results = []
+            for view in (lambda t: t.clone(), negated):
+                with torch.no_grad():
+                    results.append(list(call(*(view(t) for t in (x, y, res, w, v)))))
+                leaves = [view(t).detach().requires_grad_(True) for t in (x, y, res, w, v)]
+                outs = call(*leaves)
+                grads = torch.autograd.grad(outs, leaves, [view(x) for _ in outs], allow_unused=True)
+                results[-1] += [g for g in grads if g is not None]
+            assert len(results[0]) == len(results[1])
+            assert all(torch.equal(a, b) for a, b in zip(*results)), i

@@ -214,6 +214,11 @@ class DenseNetStage(nn.Module):
     def is_last(self) -> bool:
         return self.units[-1] == "head"
 
+    def set_epoch(self, epoch: int) -> None:
+        """The epoch that training steps belong to from now on (dropout keys of the gated head)."""
+        if hasattr(self, "ffn"):
+            self.ffn.set_epoch(epoch)
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dtype == torch.uint8:          # raw image batch: the reference's Normalize (single.py:38-42)
             x = x.float().div_(255.0)

@@ -45,6 +45,12 @@ def dropout_seed() -> int:
     return (torch.initial_seed() + 0x9E3779B97F4A7C15 * rank) % 2 ** 64
 
 
+def first_call(epoch: int) -> int:
+    """Where an epoch's dropout keys start: like the order of the data, the masks follow from the seed and the epoch, so a run that is
+    resumed at an epoch draws what the uninterrupted one drew."""
+    return (epoch % 2 ** 16) << 32
+
+
 class GatedHead(nn.Module):
     """The block in front of the classifier; ``forward`` is the portable path."""
 
@@ -58,11 +64,18 @@ class GatedHead(nn.Module):
         self.scale = nn.Parameter(torch.full((channels,), 0.1))
         self.norm_out = nn.LayerNorm(channels)
         self._rng: Optional[ops.DropoutRng] = None
+        self._epoch = 0
+
+    def set_epoch(self, epoch: int) -> None:
+        self._epoch = epoch
+        if self._rng is not None:
+            self._rng.seek(first_call(epoch))
 
     def rng(self, device) -> ops.DropoutRng:
         """The keys' generator on ``device``; it goes where the features go, and on with its sequence."""
         if self._rng is None:
             self._rng = ops.DropoutRng(dropout_seed(), device)
+            self._rng.seek(first_call(self._epoch))
         elif self._rng.state.device != torch.device(device):
             self._rng.state = self._rng.state.to(device)
         return self._rng

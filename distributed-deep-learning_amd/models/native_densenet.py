@@ -730,6 +730,7 @@ class NativeDenseNetStage(nn.Module):
         # they would draw one after the other
         self._dropout_seed = gated_head.dropout_seed()
         self._dropout_rngs: List[ops.DropoutRng] = []
+        self._epoch = 0
         self._ensure_dropout_rngs()
         self.defer_counters = False       # num_batches_tracked advanced by combine_buffer_lanes instead of per forward
         self._mb_forwarded = set()
@@ -837,7 +838,15 @@ class NativeDenseNetStage(nn.Module):
 
     def _ensure_dropout_rngs(self) -> None:
         while "head" in self.units and self.head.kind == "gated" and len(self._dropout_rngs) < len(self._buf_lanes):
-            self._dropout_rngs.append(ops.DropoutRng(self._dropout_seed, self.anchor.device, stream=len(self._dropout_rngs)))
+            rng = ops.DropoutRng(self._dropout_seed, self.anchor.device, stream=len(self._dropout_rngs))
+            rng.seek(gated_head.first_call(self._epoch))
+            self._dropout_rngs.append(rng)
+
+    def set_epoch(self, epoch: int) -> None:
+        """The epoch that training steps belong to from now on (dropout keys of the gated head)."""
+        self._epoch = epoch
+        for rng in self._dropout_rngs:
+            rng.seek(gated_head.first_call(epoch))
 
     def dropout_key(self) -> torch.Tensor:
         return self._dropout_rngs[self._buf_lane].next_key()

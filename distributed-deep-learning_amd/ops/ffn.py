@@ -113,7 +113,13 @@ class DropoutRng:
         _need(0 <= stream < 2 ** 15, f"stream must lie in [0, 2**15), got {stream}")
         seed = int(seed) % 2 ** 64
         seed = seed - 2 ** 64 if seed >= 2 ** 63 else seed          # the same 64 bits as a signed number
+        self.stream = stream
         self.state = torch.tensor([seed, stream << 48], dtype=torch.int64, device=device)
+
+    def seek(self, call: int) -> None:
+        """The next key is call number ``call`` (0 <= call < 2**48) of this generator's stream: a resumed program goes on where it was."""
+        _need(0 <= call < 2 ** 48, f"call must lie in [0, 2**48), got {call}")
+        self.state[1].fill_((self.stream << 48) + call)
 
     def keys(self, n: int) -> torch.Tensor:
         """The next ``n`` keys, [n, 2]."""

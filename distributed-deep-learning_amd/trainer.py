@@ -408,6 +408,7 @@ class Trainer:
     def _run_epoch(self, epoch: int) -> Tuple[int, int]:
         s, cfg = self.s, self.cfg
         self.train_data.set_epoch(epoch)
+        s.model.set_epoch(epoch)
         steps = len(self.train_data)
         if cfg.max_steps:
             steps = min(steps, cfg.max_steps)

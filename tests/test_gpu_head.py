@@ -168,3 +168,26 @@ def test_portable_head_moves_between_devices(dev):
     keep = torch.from_numpy(oracle.kept(state, 240, 0.25)).double().view(6, 40) / 0.75
     assert (got.cpu().double() - block64(m.cpu(), f.double(), keep)).abs().max() < 1.6e-4       # the bound of tests/test_head.py
     assert m.rng(dev).state.tolist() == [state[0], state[1] + 1]
+
+
+@pytest.mark.parametrize("graph", [False, True], ids=["eager", "graph"])
+def test_masks_follow_the_epoch(dev, graph):
+    """The keys of an epoch do not depend on how many steps ran before it, in a captured step either."""
+    from ddl import comm
+    from ddl.config import TrainConfig
+    from ddl.trainer import SingleStrategy
+    ctx = comm.CommContext(0, 1, 0, dev, "none")
+    torch.manual_seed(11)
+    strat = SingleStrategy(TrainConfig(strategy="single", batch_size=6, image_size=64, hip_graph=graph, head="gated", head_width=64,
+                                       head_dropout=0.5), ctx)
+    strat.model.train()
+    x = torch.randint(0, 256, (6, 3, 64, 64), dtype=torch.uint8, generator=torch.Generator().manual_seed(0)).to(dev)
+    y = torch.randint(0, 5, (6,), generator=torch.Generator().manual_seed(1)).to(dev)
+    for epoch, steps in ((0, 3), (1, 2), (4, 1)):
+        strat.model.set_epoch(epoch)
+        for _ in range(steps):
+            strat.train_step(x, y, 6)
+        torch.cuda.synchronize()
+        assert strat.model._dropout_rngs[0].state[1].item() == (epoch << 32) + steps
+    strat.model.ensure_buffer_lanes(1)
+    assert strat.model._dropout_rngs[1].state[1].item() == (1 << 48) + (4 << 32)

@@ -81,3 +81,28 @@ def test_dropout_keys_move_with_the_head():
     assert m.rng(torch.device("meta")).state.device.type == "meta"
     m._rng.state = torch.tensor(key)
     assert m.rng("cpu").state.tolist() == key and key[1] == 1
+
+
+def test_a_resumed_run_draws_the_masks_of_the_uninterrupted_one(tmp_dirs):
+    """Two epochs in one go, and with a stop between them: the same losses and parameters, bit for bit."""
+    from ddl.cli import run_training
+    args = [*SMALL[2:], "--batch-size", "8", "--seed", "5", "--head", "gated", "--head-width", "64", "--head-dropout", "0.5"]
+    whole = run_training("single", [*args, "--epochs", "2", "--save-every", "1"])
+    first = run_training("single", [*args, "--epochs", "1", "--save-every", "1"])
+    assert first.history[0]["loss"] == whole.history[0]["loss"]
+    second = run_training("single", [*args, "--epochs", "2", "--snapshot-job-id", first.job_id, "--snapshot-epoch", "0"])
+    assert second.history[0]["epoch"] == 1 and second.history[0]["loss"] == whole.history[1]["loss"]
+    a, b = whole.s.model.state_dict(), second.s.model.state_dict()
+    assert all(torch.equal(a[n], b[n]) for n in a)
+    key = second.s.model.ffn.rng("cpu").state[1].item()
+    assert key == (1 << 32) + 2                                       # two steps of the second epoch
+
+
+def test_seek():
+    from ddl import ops
+    rng = ops.DropoutRng(7, "cpu", stream=3)
+    rng.seek(5)
+    assert rng.next_key().tolist() == [7, (3 << 48) + 5] and rng.next_key().tolist() == [7, (3 << 48) + 6]
+    for bad in (-1, 2 ** 48):
+        with pytest.raises(ValueError):
+            rng.seek(bad)

@@ -4,8 +4,9 @@
 // streams them from memory straight into the matrix cores' A operand (lane: 16 bytes of one row), eight waves splitting k;
 // the few rows of x come out of L2 as the B operand.  The waves' sums meet in LDS in a fixed order, so the result does not
 // depend on timing.  With 16 rows a workgroup even N = 4096 gives every CU a workgroup of eight waves.
-// bf16: gated 1 x 11264 x 4096 30.5 us (185 MB at 6.0 TB/s; a large copy moves 5.1), linear 1 x 4096 x 4096 7.5 us, a launch and
-// 34 MB; fp32 30 x 4096 x 1024 9.4 us.
+// bf16: gated 1 x 11264 x 4096 39 us with all weights from memory (185 MB at 4.7 TB/s; a large copy moves 5.1), 31 to 35 where repeated
+// calls find part of them in the Infinity Cache; linear 1 x 4096 x 4096 8.5 us and 6.4 to 7.4, a launch and 34 MB; fp32
+// 30 x 4096 x 1024 10.2 us and 8.7 to 9.3.
 // Rows of x beyond M repeat row 0 (their sums are dropped).
 #include "ffn_common.h"
 #include "ffn_mma.h"

@@ -7,7 +7,8 @@ in front of it::
     y = dropout(W_down (silu(W_gate h + b_gate) * (W_up h + b_up)) + b_down)
     logits = classifier(layer_norm(f + scale * y))            # ``scale``: one learned value per channel, 0.1 at the start
 
-for fine-tuning on frozen or slowly trained features.  The block's parameters live under ``ffn.`` in the state-dict; everything
+for fine-tuning on frozen or slowly trained features.  The native engine computes it in fp32 under every ``--dtype``, like the
+linear classifier.  The block's parameters live under ``ffn.`` in the state-dict; everything
 else keeps its name, so checkpoints of either head load into the other's backbone.
 """
 from __future__ import annotations

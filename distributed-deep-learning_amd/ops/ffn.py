@@ -8,7 +8,8 @@ Together they are the residual block of a model's trunk or head::
     x, n = residual_norm(x, y, pre_weight=w, gate=g)               # join, and the next block's norm, in one pass
 
 All four are differentiable once, by a backward pass (forward-mode tangents are refused on the GPU), take float32, bfloat16 and float16 (one type per call; the vectors of ``residual_norm`` may be
-float32 beside 16-bit rows) and inputs of any strides, sum in fp32, and round a result once.  On the GPU they run the kernels of
+float32 beside 16-bit rows) and inputs of any strides, sum in fp32, and round a result once.  (16-bit gradients of products with
+more than 32 rows read dz, the gradient in front of the activation, rounded to the type, as the matrix cores want it.)  On the GPU they run the kernels of
 ``csrc/ffn_*.hip`` on the current stream and can be captured into a graph; on the CPU the same functions are plain PyTorch.
 Arguments that do not fit raise ``ValueError``; so do, on the GPU, more than 2^30 rows and products of more than 2^26 columns.
 """
@@ -76,7 +77,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     """``act(x @ weight.T + bias) + residual``: x [.., K], weight [N, K], bias [N], residual [.., N].
 
     Bias, activation and residual are the product's epilogue.  Training keeps x, weight and - with an activation - the fp32
-    sums in front of it, so that the gradients round once."""
+    sums in front of it, so that the activation's slope is taken from unrounded sums.  On the GPU an operand that the kernels cannot
+    read in place (a width off 16 bytes, strides) is kept as the copy they read: a second copy of such a weight until ``backward``,
+    and the gradients are those of the values at the call even if the tensor is changed in place between."""
     a = act_id(activation)
     if x.is_cuda:
         return require_ext().linear(x, weight, bias, residual, a)
@@ -89,7 +92,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
                  b_up: Optional[torch.Tensor] = None, activation: str = "silu") -> torch.Tensor:
     """``act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up)``: x [.., K], weights [F, K], both biases [F] or none.
 
-    Both projections are one kernel; neither is written to memory at inference.  Training keeps both in fp32."""
+    Both projections are one kernel; neither is written to memory at inference.  Training keeps both in fp32, and x and the weights
+    as ``linear`` does."""
     a = act_id(activation)
     if x.is_cuda:
         return require_ext().gated_linear(x, w_gate, w_up, b_gate, b_up, a)

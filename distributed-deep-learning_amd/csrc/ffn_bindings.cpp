@@ -10,6 +10,7 @@
 #include "ffn_misc.h"
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <string>
 
@@ -483,6 +484,26 @@ struct Needs {
     return (given >> i & 1) && ctx->needs_input_grad((size_t)__builtin_popcountll(given & ((1ll << i) - 1)));
   }
 };
+// PyTorch hands a gradient to the next node on the stream where that node was made.  A leaf's accumulation node is made by the leaf's first
+// use and lives as long as a result of it (or a hook): an eager result that is alive puts it on the default stream, and to wait for that
+// stream ends a capture, and the process with it.  So a backward pass that is being captured refuses such a gradient, before anything
+// is launched for it.
+void no_capture_onto_default_stream(const char* op) {
+  const auto here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA();
+  if (here.unwrap().id() == 0) return;                               // the default stream itself: nothing is captured on it
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  DDL_HIP_CHECK(hipStreamIsCapturing(here.stream(), &status));
+  const auto node = torch::autograd::get_current_node();
+  if (status == hipStreamCaptureStatusNone || !node) return;
+  for (uint32_t i = 0; i < node->num_outputs(); ++i) {
+    const auto& next = node->next_edge(i).function;
+    if (!next || !node->task_should_compute_output(i)) continue;
+    const auto stream = next->stream();
+    TORCH_CHECK(!stream.has_value() || stream->id() != 0, op, ": this backward pass is being captured, and a gradient goes to ",
+                next->name(), " on the default stream, which would break the capture.  An eager result of the same tensor is alive, or a "
+                "hook holds its node: free it before the capture, or use the tensor on the capturing stream first");
+  }
+}
 struct LinearFn : torch::autograd::Function<LinearFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptT& b, const OptT& res, int64_t act) {
     at::AutoDispatchBelowADInplaceOrView below;
@@ -500,6 +521,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     no_second_derivative("linear");
     if (!grads[0].defined()) return variable_list(5);
     no_tangent(grads[0], "linear");
+    no_capture_onto_default_stream("linear");
     const auto saved = ctx->get_saved_variables();
     const Needs need(ctx);
     ddl::DeviceGuard guard(grads[0].device());
@@ -564,6 +586,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     no_second_derivative("gated_linear");
     if (!grads[0].defined()) return variable_list(6);
     no_tangent(grads[0], "gated_linear");
+    no_capture_onto_default_stream("gated_linear");
     const auto s = ctx->get_saved_variables();
     const Needs need(ctx);
     ddl::DeviceGuard guard(grads[0].device());
@@ -628,6 +651,7 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
     no_second_derivative("dropout");
     if (!grads[0].defined()) return variable_list(4);
     no_tangent(grads[0], "dropout");
+    no_capture_onto_default_stream("dropout");
     const Needs need(ctx);
     Tensor dx;
     if (need(0))
@@ -851,6 +875,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
     }
     variable_list out(10);
     if (!dr.defined() && !dh.defined()) return out;
+    no_capture_onto_default_stream("residual_norm");
     const Needs need(ctx);
     NormGrads g = norm_backward(in, v[7], dr, dh, need(0), need(1), need(2), need(3), need(4), need(5), need(6));
     out[0] = g.dx;

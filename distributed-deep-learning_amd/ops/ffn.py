@@ -121,7 +121,8 @@ class DropoutRng:
         self.state = torch.tensor([seed, stream << 48], dtype=torch.int64, device=device)
 
     def seek(self, call: int) -> None:
-        """The next key is call number ``call`` (0 <= call < 2**48) of this generator's stream: a resumed program goes on where it was."""
+        """The next key is call number ``call`` (0 <= call < 2**48) of this generator's stream: a resumed program goes on where it was.
+        (Between captured steps, not in one: every replay would seek again.)"""
         _need(0 <= call < 2 ** 48, f"call must lie in [0, 2**48), got {call}")
         self.state[1].fill_((self.stream << 48) + call)
 

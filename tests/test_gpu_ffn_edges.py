@@ -400,3 +400,34 @@ def test_negated_views(dev):
                 results[-1] += [g for g in grads if g is not None]
             assert len(results[0]) == len(results[1])
             assert all(torch.equal(a, b) for a, b in zip(*results)), i
+
+
+# ---- captures ----------------------------------------------------------------------------------------------------------------------
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("op", ["linear", "gated_linear", "dropout", "residual_norm"])
+def test_a_captured_backward_beside_an_eager_result(dev, op):
+    """An eager result of the leaf on the default stream is alive: the captured backward pass raises instead of ending the process,
+    and works once the result is gone."""
+    from ddl import ops
+    x, w = rnd(dev, torch.float32, 40, 16).requires_grad_(True), rnd(dev, torch.float32, 16, 16, seed=1).requires_grad_(True)
+    key = torch.tensor([1, 2], device=dev)
+    call = {"linear": lambda x: ops.linear(x, w, activation="silu"), "gated_linear": lambda x: ops.gated_linear(x, w, w),
+            "dropout": lambda x: ops.dropout(x, 0.3, key), "residual_norm": lambda x: ops.residual_norm(x, pre_weight=w[0].detach())[1]}[op]
+    dy = rnd(dev, torch.float32, 40, 16, seed=2)
+    (want,) = torch.autograd.grad(call(x), x, dy)
+    held = call(x)                                                   # x's accumulation node stays on the default stream
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = call(x)
+        with pytest.raises(RuntimeError, match="default stream"):
+            torch.autograd.grad(y, x, dy)
+    del y, held, graph
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (dx,) = torch.autograd.grad(call(x), x, dy)
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(dx, want)
+        (again,) = torch.autograd.grad(call(x), x, dy)
+        assert torch.equal(again, want)
